@@ -127,5 +127,6 @@ RopeTables rope_tables(const Tensor& cos, const Tensor& sin, int64_t seq, int64_
 Tensor lora_grad_a(const Tensor& q, const Tensor& scale, const Tensor& gm, int64_t r2, int64_t q_bit);
 void bind_ops(pybind11::module_& m);
 void bind_blocks(pybind11::module_& m);
+void bind_forms(pybind11::module_& m);
 
 }  // namespace hyc_host

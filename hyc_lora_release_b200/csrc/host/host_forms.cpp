@@ -1,0 +1,138 @@
+// Operators of other layer forms: norms and rotation of query and key heads.
+#include "host.h"
+
+namespace hyc_host {
+
+static int elem_type(at::ScalarType t) { return t == at::kBFloat16 ? HYC_BF16 : t == at::kHalf ? HYC_F16 : t == at::kFloat ? HYC_F32 : -1; }
+static int elem_type(const Tensor& t, const char* what) {
+  const int e = elem_type(t.scalar_type());
+  TORCH_CHECK_VALUE(e >= 0, what, " must be bf16, fp16 or fp32, got ", t.scalar_type());
+  return e;
+}
+static bool on16(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
+
+// ---- norms and rotation of query and key heads
+// [batch, seq, heads, d] with adjacent channels and 16-byte rows, as it is or as a copy; the strides of its first three dimensions
+static Tensor head_view(const Tensor& t_in, int64_t (&stride)[3]) {
+  Tensor t = t_in;
+  const int64_t e = 16 / t.element_size();
+  auto fits = [&]() {
+    if (t.stride(3) != 1 || !on16(t)) return false;
+    for (int i = 0; i < 3; ++i) {
+      stride[i] = t.size(i) > 1 ? t.stride(i) : 0;
+      if (stride[i] % e != 0) return false;
+    }
+    return true;
+  };
+  if (t.numel() > 0 && !fits()) {
+    t = t.contiguous();
+    if (!fits()) { t = t.clone(); fits(); }      // (contiguous, but begins off a 16-byte boundary)
+  }
+  return t;
+}
+// a table of `rows` angles as [rows, >= half]
+static Tensor angle_table(const Tensor& t_in, int64_t half, const char* what) {
+  TORCH_CHECK_VALUE(t_in.dim() >= 2 && t_in.numel() == t_in.size(-2) * t_in.size(-1) && t_in.size(-1) >= half, what,
+                    " must be a [positions, >= rotary_dim / 2] table, got shape ", t_in.sizes());
+  Tensor t = t_in.dim() == 2 ? t_in : t_in.reshape({t_in.size(-2), t_in.size(-1)});
+  if (elem_type(t.scalar_type()) < 0) t = t.to(at::kFloat);
+  if (t.numel() > 0 && (t.stride(1) != 1 || !on16(t) || (t.size(0) > 1 && t.stride(0) % (16 / t.element_size()) != 0)))
+    t = t.narrow(1, 0, half).clone(at::MemoryFormat::Contiguous);
+  return t;
+}
+
+namespace {
+struct QkNorm {
+  hyc_qk_norm a = {};
+  Tensor hold[8];
+
+  void inputs(const Tensor& q, const Tensor& k, const Tensor& qw, const Tensor& kw, const Tensor& cos_in, const Tensor& sin_in, double eps,
+              const OptTensor& pos, const std::optional<int64_t>& rotary_dim) {
+    TORCH_CHECK_VALUE(q.dim() == 4 && k.dim() == 4 && q.size(0) == k.size(0) && q.size(1) == k.size(1) && q.size(3) == k.size(3),
+                      "q and k must be [batch, seq_len, heads, head_dim] with the same batch, length and head size, got ", q.sizes(), " and ", k.sizes());
+    TORCH_CHECK_VALUE(q.scalar_type() == k.scalar_type(), "q and k must have one type, got ", q.scalar_type(), " and ", k.scalar_type());
+    const int64_t d = q.size(3), rot = rotary_dim.value_or(d);
+    TORCH_CHECK_VALUE(d >= 16 && d % 16 == 0 && d <= 512, "head_dim must be a multiple of 16 up to 512, got ", d);
+    TORCH_CHECK_VALUE(rot >= 16 && rot % 16 == 0 && rot <= d, "rotary_dim must be a multiple of 16 from 16 to head_dim, got ", rot);
+    TORCH_CHECK_VALUE(q.size(2) >= 1 && k.size(2) >= 1, "q and k need a head each");
+    TORCH_CHECK_VALUE(q.size(2) <= 65536 && k.size(2) <= 65536 && q.size(0) * q.size(1) <= 0x7fffffffll, "more than 65536 heads or 2^31 - 1 tokens");
+    TORCH_CHECK_VALUE(qw.numel() == d && kw.numel() == d && qw.scalar_type() == kw.scalar_type(),
+                      "q_weight and k_weight must have head_dim = ", d, " entries and one type");
+    a.batch = q.size(0); a.seq = q.size(1); a.head_dim = (int)d; a.rotary_dim = (int)rot; a.eps = (float)eps;
+    a.heads[0] = (int)q.size(2); a.heads[1] = (int)k.size(2);
+    a.type = elem_type(q, "q and k"); a.w_type = elem_type(qw, "q_weight and k_weight");
+    hold[0] = head_view(q, a.x_stride[0]); hold[1] = head_view(k, a.x_stride[1]);
+    const Tensor* w[2] = {&qw, &kw};
+    for (int i = 0; i < 2; ++i) {
+      Tensor& c = hold[2 + i];
+      c = w[i]->contiguous();
+      if (!on16(c)) c = c.clone();
+      a.x[i] = data(hold[i]); a.weight[i] = data(c);
+    }
+    Tensor cos = angle_table(cos_in, rot / 2, "cos"), sin = angle_table(sin_in, rot / 2, "sin");
+    TORCH_CHECK_VALUE(cos.size(0) == sin.size(0), "cos and sin must have the same number of positions");
+    if (sin.scalar_type() != cos.scalar_type()) { cos = cos.to(at::kFloat); sin = sin.to(at::kFloat); }
+    a.cos_t = data(cos); a.sin_t = data(sin); a.ld_cos = cos.stride(0); a.ld_sin = sin.stride(0);
+    a.table_rows = cos.size(0); a.table_type = elem_type(cos.scalar_type());
+    hold[4] = cos; hold[5] = sin;
+    if (cos.size(0) <= 1) a.ld_cos = a.ld_sin = (rot / 2 + 7) / 8 * 8;
+    if (given(pos)) {
+      TORCH_CHECK_VALUE(pos->dim() == 2 && (pos->size(0) == a.batch || pos->size(0) == 1) && pos->size(1) == a.seq &&
+                            (pos->scalar_type() == at::kLong || pos->scalar_type() == at::kInt),
+                        "position_ids must be int32 or int64 [batch or 1, seq_len], got ", pos->scalar_type(), " ", pos->sizes());
+      a.position_ids = data(*pos);
+      a.pos_is_int64 = pos->scalar_type() == at::kLong;
+      a.pos_stride[0] = pos->size(0) == 1 ? 0 : pos->stride(0);
+      a.pos_stride[1] = pos->stride(1);
+    } else {
+      TORCH_CHECK_VALUE(cos.size(0) >= a.seq, "the rotary tables have ", cos.size(0), " positions, the sequence ", a.seq);
+    }
+  }
+};
+}  // namespace
+
+static std::tuple<Tensor, Tensor> qk_norm_rope_forward(const Tensor& q, const Tensor& k, const Tensor& qw, const Tensor& kw, const Tensor& cos,
+                                                       const Tensor& sin, double eps, const OptTensor& pos, const std::optional<int64_t>& rotary_dim) {
+  require_cuda({&q, &k, &qw, &kw, &cos, &sin, opt(pos)});
+  OnDevice on(q);
+  QkNorm n;
+  n.inputs(q, k, qw, kw, cos, sin, eps, pos, rotary_dim);
+  const Tensor oq = empty(q.sizes(), q, q.scalar_type()), ok = empty(k.sizes(), k, k.scalar_type());
+  n.a.out[0] = data(oq); n.a.out[1] = data(ok);
+  check(hyc_qk_norm_rope_fwd(&n.a, on.stream), "hyc_qk_norm_rope_fwd");
+  return {oq, ok};
+}
+
+static std::tuple<Tensor, Tensor, OptTensor, OptTensor> qk_norm_rope_backward(const Tensor& dq, const Tensor& dk, const Tensor& q, const Tensor& k,
+                                                                              const Tensor& qw, const Tensor& kw, const Tensor& cos, const Tensor& sin,
+                                                                              double eps, const OptTensor& pos, const std::optional<int64_t>& rotary_dim,
+                                                                              bool needs_weight_grad) {
+  require_cuda({&q, &k, &dq, &dk, &qw, &kw, &cos, &sin, opt(pos)});
+  OnDevice on(q);
+  QkNorm n;
+  n.inputs(q, k, qw, kw, cos, sin, eps, pos, rotary_dim);
+  TORCH_CHECK_VALUE(dq.sizes() == q.sizes() && dk.sizes() == k.sizes(), "the gradients must have the shapes ", q.sizes(), " and ", k.sizes(), ", got ",
+                    dq.sizes(), " and ", dk.sizes());
+  TORCH_CHECK_VALUE(dq.scalar_type() == q.scalar_type() && dk.scalar_type() == q.scalar_type(), "the gradients must have the type of q and k, ", q.scalar_type());
+  n.hold[6] = head_view(dq, n.a.dy_stride[0]); n.hold[7] = head_view(dk, n.a.dy_stride[1]);
+  n.a.dy[0] = data(n.hold[6]); n.a.dy[1] = data(n.hold[7]);
+  const Tensor oq = empty(q.sizes(), q, q.scalar_type()), ok = empty(k.sizes(), k, k.scalar_type());
+  n.a.out[0] = data(oq); n.a.out[1] = data(ok);
+  OptTensor wq, wk;
+  Tensor ws;
+  size_t bytes = 0;
+  if (needs_weight_grad) {
+    wq = empty(qw.sizes(), qw, qw.scalar_type()); wk = empty(kw.sizes(), kw, kw.scalar_type());
+    bytes = hyc_qk_norm_rope_workspace_bytes(n.a.head_dim);
+    ws = empty({(int64_t)bytes}, q, at::kByte);
+  }
+  check(hyc_qk_norm_rope_bwd(&n.a, data(wq), data(wk), data(ws), bytes, on.stream), "hyc_qk_norm_rope_bwd");
+  return {oq, ok, wq, wk};
+}
+
+void bind_forms(pybind11::module_& m) {
+  m.def("qk_norm_rope_forward", &qk_norm_rope_forward);
+  m.def("qk_norm_rope_backward", &qk_norm_rope_backward);
+}
+
+}  // namespace hyc_host

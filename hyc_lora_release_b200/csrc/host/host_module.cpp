@@ -20,4 +20,5 @@ PYBIND11_MODULE(_hyc_host, m) {
   });
   bind_ops(m);
   bind_blocks(m);
+  bind_forms(m);
 }

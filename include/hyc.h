@@ -37,6 +37,8 @@ enum {
   HYC_ERR_UNSUPPORTED = -8  /* feature not available in this build */
 };
 
+enum { HYC_BF16 = 0, HYC_F16 = 1, HYC_F32 = 2 };   /* element types, where an entry point takes more than bf16 */
+
 const char* hyc_strerror(int code);
 int hyc_last_cuda_error(void);   /* cudaError_t of the last HYC_ERR_LAUNCH, else 0 */
 int hyc_version(void);
@@ -504,6 +506,33 @@ size_t hyc_lora_grad_a_workspace_bytes(int T, int H, int R2);
 int hyc_lora_grad_a_dequant(const void* q, const void* scale, const void* gm, int64_t ldg, int R2,
                             int T, int H, int q_bit, void* out, void* workspace, size_t workspace_bytes,
                             void* stream);
+
+/* ---- norms of query and key heads with the rotary embedding -------------------------
+ *
+ * For every head x of q ([batch, seq, heads[0], head_dim]) and k ([batch, seq, heads[1], head_dim]):
+ *   n = x / sqrt(mean(x^2) + eps) * weight,   out = n with its first rotary_dim channels turned in the rotate-half form by the
+ *   angles of the token's position, the others as they are.  fp32 inside, rounded once.
+ * Index 0 is q, 1 is k.  x, dy: any strides (elements: batch, token, head; multiples of 16 bytes; dy may have strides of 0),
+ * channels adjacent, on 16 bytes; out contiguous; weight [head_dim] of w_type.  head_dim and rotary_dim: multiples of 16,
+ * head_dim <= 512.  cos_t / sin_t: table_rows rows of at least rotary_dim / 2 values of table_type (the columns behind those are not
+ * read), row strides multiples of 16 bytes.  position_ids: int32 or int64 per token with strides pos_stride (batch, token), or
+ * null: a token's index in its sequence.  A position outside of the tables gives NaN in the channels that are turned.
+ * fwd: out = the turned heads.  bwd: x = the heads as forward read them, dy = the gradients of its results, out = the gradients of
+ * its inputs; dweight_q / dweight_k [head_dim] of w_type receive the gradients of the weights, both null: not wanted; workspace of
+ * hyc_qk_norm_rope_workspace_bytes(head_dim) for them. */
+typedef struct {
+  const void* x[2]; const void* dy[2]; const void* weight[2]; void* out[2];
+  int64_t x_stride[2][3], dy_stride[2][3];
+  const void* cos_t; const void* sin_t; int64_t ld_cos, ld_sin, table_rows;
+  const void* position_ids; int64_t pos_stride[2]; int pos_is_int64;
+  int64_t batch, seq;
+  int heads[2], head_dim, rotary_dim;
+  int type, w_type, table_type;
+  float eps;
+} hyc_qk_norm;
+int hyc_qk_norm_rope_fwd(const hyc_qk_norm* args, void* stream);
+size_t hyc_qk_norm_rope_workspace_bytes(int head_dim);
+int hyc_qk_norm_rope_bwd(const hyc_qk_norm* args, void* dweight_q, void* dweight_k, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
