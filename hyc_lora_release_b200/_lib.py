@@ -72,6 +72,9 @@ SIGNATURES = {
     "hyc_qk_norm_rope_fwd": (_i, [_p, _p]),
     "hyc_qk_norm_rope_workspace_bytes": (_z, [_i]),
     "hyc_qk_norm_rope_bwd": (_i, [_p, _p, _p, _p, _z, _p]),
+    "hyc_softmax_relative_bias_fwd": (_i, [_p, _p]),
+    "hyc_softmax_relative_bias_workspace_bytes": (_z, [_p]),
+    "hyc_softmax_relative_bias_bwd": (_i, [_p, _p, _p, _z, _p]),
     "hyc_dequant_nf4": (_i, [_p, _p, _p, _p, _p, _p, _i, _f, _l, _i, _p, _p]),
     "hyc_gemm_bf16_tcgen05": (_i, [_p, _p, _i, _i, _i, _i, _p, _p, _i, _p, _p, _i,
                                    _p, _p, _l, _l, _p, _p, _l, _l, _p, _p, _p, _p]),

@@ -130,7 +130,68 @@ static std::tuple<Tensor, Tensor, OptTensor, OptTensor> qk_norm_rope_backward(co
   return {oq, ok, wq, wk};
 }
 
+// ---- softmax with a learned bias per bucket of relative positions
+static hyc_relative_bias relative_bias_args(const Tensor& x, double scale, const Tensor& edges, bool both, bool causal, int64_t q_offset) {
+  TORCH_CHECK_VALUE(x.dim() == 4, "expected a [batch, heads, n, S] map, got shape ", x.sizes());
+  TORCH_CHECK_VALUE(x.size(3) >= 1, "the last dimension is empty (shape ", x.sizes(), ")");
+  TORCH_CHECK_VALUE(x.size(3) <= HYC_RELATIVE_BIAS_MAX_COLS, "rows of more than ", (int)HYC_RELATIVE_BIAS_MAX_COLS, " columns");
+  TORCH_CHECK_VALUE(x.size(1) >= 1, "the map has no heads");
+  TORCH_CHECK_VALUE(x.size(0) * x.size(1) * x.size(2) <= 0x7fffffffll, "more than 2^31 - 1 rows");
+  TORCH_CHECK_VALUE(std::abs(q_offset) < (1ll << 29), "q_offset is out of range: ", q_offset);
+  TORCH_CHECK_VALUE(!edges.is_cuda() && edges.scalar_type() == at::kInt && edges.dim() == 1 && edges.is_contiguous() && edges.numel() >= 1,
+                    "the buckets' edges must be an int32 vector on the host");
+  hyc_relative_bias a = {};
+  a.batch = x.size(0); a.heads = (int)x.size(1); a.n = x.size(2); a.cols = x.size(3); a.q_offset = q_offset;
+  a.host_edges = (const int32_t*)edges.data_ptr(); a.side = (int)edges.numel(); a.both = both; a.causal = causal;
+  a.type = elem_type(x, "the map"); a.scale = (float)scale;
+  return a;
+}
+
+static Tensor softmax_relative_bias_forward(const Tensor& scores, double scale, const Tensor& table, const Tensor& edges, bool both, const OptTensor& mask,
+                                            bool causal, int64_t q_offset, bool inplace) {
+  require_cuda({&scores, &table, opt(mask)});
+  OnDevice on(scores);
+  hyc_relative_bias a = relative_bias_args(scores, scale, edges, both, causal, q_offset);
+  TORCH_CHECK_VALUE(!inplace || scores.is_contiguous(), "inplace needs contiguous scores");
+  TORCH_CHECK_VALUE(table.dim() == 2 && table.size(0) == (both ? 2 : 1) * a.side && table.size(1) == a.heads, "the table must be [", (both ? 2 : 1) * a.side,
+                    " buckets, ", a.heads, " heads], got ", table.sizes());
+  const Tensor x = scores.contiguous(), t = table.contiguous();
+  const Tensor out = inplace ? x : empty(x.sizes(), x, x.scalar_type());
+  Tensor mk;
+  if (given(mask)) {
+    mk = *mask;
+    TORCH_CHECK_VALUE(mk.dim() == 4 && mk.size(3) == a.cols && (mk.size(2) == 1 || mk.size(2) == a.n) && (mk.size(1) == 1 || mk.size(1) == a.heads) &&
+                          (mk.size(0) == 1 || mk.size(0) == a.batch),
+                      "attention_mask must be [b or 1, h or 1, n or 1, S], got ", mk.sizes());
+    a.mask_type = elem_type(mk, "attention_mask");
+    if (mk.stride(3) != 1) mk = mk.contiguous();
+    a.mask = data(mk);
+    a.mask_b = mk.size(0) == 1 ? 0 : mk.stride(0); a.mask_h = mk.size(1) == 1 ? 0 : mk.stride(1); a.mask_row = mk.size(2) == 1 ? 0 : mk.stride(2);
+  }
+  a.x = data(x); a.out = data(out); a.table = data(t); a.table_type = elem_type(t, "the table");
+  check(hyc_softmax_relative_bias_fwd(&a, on.stream), "hyc_softmax_relative_bias_fwd");
+  return inplace ? scores : out;
+}
+
+static std::tuple<Tensor, Tensor> softmax_relative_bias_backward(const Tensor& map, const Tensor& grad, double scale, const Tensor& edges, bool both,
+                                                                 bool causal, int64_t q_offset) {
+  require_cuda({&map, &grad});
+  OnDevice on(map);
+  hyc_relative_bias a = relative_bias_args(map, scale, edges, both, causal, q_offset);
+  TORCH_CHECK_VALUE(grad.sizes() == map.sizes() && grad.scalar_type() == map.scalar_type(), "the gradient must have the map's shape and type, ",
+                    map.scalar_type(), " ", map.sizes(), ", got ", grad.scalar_type(), " ", grad.sizes());
+  const Tensor x = map.contiguous(), g = grad.contiguous();
+  const Tensor out = empty(x.sizes(), x, x.scalar_type()), table = empty({(both ? 2 : 1) * a.side, a.heads}, x, at::kFloat);
+  a.x = data(x); a.grad = data(g); a.out = data(out);
+  const size_t bytes = hyc_softmax_relative_bias_workspace_bytes(&a);
+  const Tensor ws = empty({(int64_t)bytes}, x, at::kByte);
+  check(hyc_softmax_relative_bias_bwd(&a, (float*)data(table), data(ws), bytes, on.stream), "hyc_softmax_relative_bias_bwd");
+  return {out, table};
+}
+
 void bind_forms(pybind11::module_& m) {
+  m.def("softmax_relative_bias_forward", &softmax_relative_bias_forward);
+  m.def("softmax_relative_bias_backward", &softmax_relative_bias_backward);
   m.def("qk_norm_rope_forward", &qk_norm_rope_forward);
   m.def("qk_norm_rope_backward", &qk_norm_rope_backward);
 }

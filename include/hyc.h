@@ -534,6 +534,32 @@ int hyc_qk_norm_rope_fwd(const hyc_qk_norm* args, void* stream);
 size_t hyc_qk_norm_rope_workspace_bytes(int head_dim);
 int hyc_qk_norm_rope_bwd(const hyc_qk_norm* args, void* dweight_q, void* dweight_k, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- softmax with a learned bias per bucket of relative positions -------------------
+ *
+ * fwd: out[b, h, i, j] = softmax_j(scale * x[b, h, i, j] + table[bucket(j - i - q_offset), h] + mask[b, h, i, j]), x and out contiguous
+ * [batch, heads, n, cols] of `type` (out may be x); causal: only columns j <= i + q_offset count, the others are not read and become
+ * 0.  A row in which nothing counts (no column, or -infinity everywhere) becomes 0.  fp32 inside, rounded once.
+ *   host_edges: `side` ascending lower edges in HOST memory, the first 0, the last at most HYC_RELATIVE_BIAS_MAX_DISTANCE; k(r) = the number
+ *   of edges <= r, less one.  bucket(d) = k(-d) for d <= 0; for d > 0: side + k(d) if both != 0, else 0.
+ *   table [side or 2 side, heads] of table_type; mask (or null) of mask_type, element strides of batch, head and row (0: shared),
+ *   columns adjacent.  cols <= HYC_RELATIVE_BIAS_MAX_COLS.
+ * bwd: x = the probabilities, grad = the gradient of them (contiguous): ds = x * (grad - rowsum(x * grad)), out = scale * ds,
+ *   dtable [side or 2 side, heads] fp32 = the sums of ds over the places of a bucket; table and mask are not read.  workspace:
+ *   hyc_softmax_relative_bias_workspace_bytes(args) bytes, on 16 bytes. */
+enum { HYC_RELATIVE_BIAS_MAX_COLS = 131072, HYC_RELATIVE_BIAS_MAX_DISTANCE = 8192 };
+typedef struct {
+  const void* x; const void* grad; void* out;
+  const void* table; const void* mask; int64_t mask_b, mask_h, mask_row;
+  const int32_t* host_edges;
+  int64_t batch, n, cols, q_offset;
+  int heads, side, both, causal;
+  int type, table_type, mask_type;
+  float scale;
+} hyc_relative_bias;
+int hyc_softmax_relative_bias_fwd(const hyc_relative_bias* args, void* stream);
+size_t hyc_softmax_relative_bias_workspace_bytes(const hyc_relative_bias* args);
+int hyc_softmax_relative_bias_bwd(const hyc_relative_bias* args, float* dtable, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
