@@ -75,6 +75,10 @@ SIGNATURES = {
     "hyc_softmax_relative_bias_fwd": (_i, [_p, _p]),
     "hyc_softmax_relative_bias_workspace_bytes": (_z, [_p]),
     "hyc_softmax_relative_bias_bwd": (_i, [_p, _p, _p, _z, _p]),
+    "hyc_linear_act_tcgen05": (_i, [_p, _p]),
+    "hyc_linear_act_dpre_workspace_bytes": (_z, [_i]),
+    "hyc_linear_act_dpre": (_i, [_p, _l, _p, _p, _p, _l, _i, _i, _i, _p, _z, _p]),
+    "hyc_linear_status": (_i, [_p]),
     "hyc_dequant_nf4": (_i, [_p, _p, _p, _p, _p, _p, _i, _f, _l, _i, _p, _p]),
     "hyc_gemm_bf16_tcgen05": (_i, [_p, _p, _i, _i, _i, _i, _p, _p, _i, _p, _p, _i,
                                    _p, _p, _l, _l, _p, _p, _l, _l, _p, _p, _p, _p]),

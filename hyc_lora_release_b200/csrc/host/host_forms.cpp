@@ -189,7 +189,123 @@ static std::tuple<Tensor, Tensor> softmax_relative_bias_backward(const Tensor& m
   return {out, table};
 }
 
+// ---- products with bias, activation and residual
+// [.., n] as rows of n adjacent elements on 16 bytes with one stride, as it is or as a copy
+static Tensor rows_of(const Tensor& t_in, int64_t& ld) {
+  const int64_t n = t_in.size(-1);
+  auto rows = [&](const Tensor& t) { return t.dim() == 2 ? t : t.reshape({-1, n}); };
+  Tensor t = t_in.numel() == 0 ? t_in.new_empty({t_in.numel() / n, n}) : rows(t_in);
+  auto fits = [&]() {
+    ld = t.size(0) > 1 ? t.stride(0) : n;
+    return t.stride(1) == 1 && ld % 8 == 0 && ld >= n && on16(t);
+  };
+  if (t.numel() > 0 && !fits()) {
+    t = t.clone(at::MemoryFormat::Contiguous);
+    fits();
+  }
+  if (t.numel() == 0) ld = n;
+  return t;
+}
+static void check_linear(const Tensor& x, const Tensor& w, const char* what) {
+  TORCH_CHECK_VALUE(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf, what, " must be bf16 or fp16, got ", x.scalar_type());
+  TORCH_CHECK_VALUE(w.dim() == 2 && w.scalar_type() == x.scalar_type(), "weight must be a [out, in] matrix of the type ", x.scalar_type(), ", got ", w.scalar_type(),
+                    " ", w.sizes());
+  TORCH_CHECK_VALUE(w.size(0) >= 8 && w.size(1) >= 8 && w.size(0) % 8 == 0 && w.size(1) % 8 == 0 && w.size(0) <= (1 << 24) && w.size(1) <= (1 << 24),
+                    "both sizes of the weight must be multiples of 8 up to 2^24, got ", w.sizes());
+}
+static at::DimVector with_last(const Tensor& like, int64_t n) {
+  at::DimVector s(like.sizes().begin(), like.sizes().end());
+  s.back() = n;
+  return s;
+}
+
+static std::tuple<Tensor, OptTensor> linear_act_forward(const Tensor& x, const Tensor& w, const OptTensor& bias, int64_t act, const OptTensor& residual,
+                                                        bool save_pre) {
+  require_cuda({&x, &w, opt(bias), opt(residual)});
+  check_linear(x, w, "x");
+  const int64_t n = w.size(0), k = w.size(1);
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) == k, "x must be [.., ", k, "] for this weight, got ", x.sizes());
+  TORCH_CHECK_VALUE(x.numel() / k <= 0x3fffffffll, "more than 2^30 - 1 rows");
+  const at::DimVector shape = with_last(x, n);
+  TORCH_CHECK_VALUE(!given(bias) || (bias->numel() == n && bias->scalar_type() == x.scalar_type()), "bias must have ", n, " entries of the type ", x.scalar_type());
+  TORCH_CHECK_VALUE(!given(residual) || (residual->sizes() == at::IntArrayRef(shape) && residual->scalar_type() == x.scalar_type()),
+                    "residual must have the result's shape ", at::IntArrayRef(shape), " and the type ", x.scalar_type());
+  OnDevice on(x);
+  hyc_linear a = {};
+  const Tensor xr = rows_of(x, a.ld_a), wr = rows_of(w, a.ld_b), b = given(bias) ? bias->contiguous() : Tensor();
+  Tensor res;
+  if (given(residual)) res = rows_of(*residual, a.ld_res);
+  const Tensor out = empty(shape, x, x.scalar_type());
+  OptTensor pre;
+  if (save_pre) pre = empty(shape, x, x.scalar_type());
+  a.a = data(xr); a.b = data(wr); a.bias = data(b); a.residual = data(res); a.pre = data(pre); a.out = data(out);
+  a.rows = xr.size(0); a.cols = (int)n; a.depth = (int)k; a.type = elem_type(x.scalar_type()); a.act = (int)act;
+  check(hyc_linear_act_tcgen05(&a, on.stream), "hyc_linear_act_tcgen05");
+  return {out, pre};
+}
+
+static std::tuple<OptTensor, OptTensor, OptTensor> linear_act_backward(const Tensor& dy, const Tensor& x, const Tensor& w, int64_t act, const OptTensor& pre,
+                                                                       bool need_x, bool need_w, bool need_b) {
+  require_cuda({&dy, &x, &w, opt(pre)});
+  check_linear(x, w, "x");
+  const int64_t n = w.size(0), k = w.size(1);
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) == k, "x must be [.., ", k, "] for this weight, got ", x.sizes());
+  const at::DimVector shape = with_last(x, n);
+  TORCH_CHECK_VALUE(dy.sizes() == at::IntArrayRef(shape) && dy.scalar_type() == x.scalar_type(), "dy must be ", at::IntArrayRef(shape), " of the type ",
+                    x.scalar_type(), ", got ", dy.scalar_type(), " ", dy.sizes());
+  TORCH_CHECK_VALUE(act == HYC_ACT_NONE || (given(pre) && pre->sizes() == at::IntArrayRef(shape) && pre->scalar_type() == x.scalar_type()),
+                    "an activation's backward pass needs pre as forward saved it");
+  TORCH_CHECK_VALUE(x.numel() / k <= 0x3fffffffll, "more than 2^30 - 1 rows");
+  OnDevice on(x);
+  OptTensor dx, dw, db;
+  const int64_t rows = x.numel() / k;
+  const int type = elem_type(x.scalar_type());
+  int64_t ld = 0;
+  Tensor g = rows_of(dy, ld);
+  if (act != HYC_ACT_NONE || need_b) {
+    Tensor d, ws;
+    size_t bytes = 0;
+    if (act != HYC_ACT_NONE) d = empty({rows, n}, x, x.scalar_type());
+    if (need_b) {
+      db = empty({n}, x, x.scalar_type());
+      bytes = hyc_linear_act_dpre_workspace_bytes((int)n);
+      ws = empty({(int64_t)bytes}, x, at::kByte);
+    }
+    const Tensor p = act != HYC_ACT_NONE ? pre->contiguous() : Tensor();
+    const Tensor pa = p.defined() && p.numel() > 0 && !on16(p) ? p.clone() : p;
+    check(hyc_linear_act_dpre(data(g), ld, data(pa), data(d), data(db), rows, (int)n, type, (int)act, data(ws), bytes, on.stream), "hyc_linear_act_dpre");
+    if (d.defined()) { g = d; ld = n; }
+  }
+  hyc_linear a = {};
+  a.a = data(g); a.ld_a = ld; a.b_mn = 1; a.type = type;
+  if (need_x) {
+    dx = empty(x.sizes(), x, x.scalar_type());
+    const Tensor wr = rows_of(w, a.ld_b);
+    a.b = data(wr); a.out = data(dx); a.rows = rows; a.cols = (int)k; a.depth = (int)n;
+    check(hyc_linear_act_tcgen05(&a, on.stream), "hyc_linear_act_tcgen05");
+  }
+  if (need_w) {
+    dw = empty(w.sizes(), w, w.scalar_type());
+    if (rows == 0) {
+      dw->zero_();
+    } else {
+      const Tensor xr = rows_of(x, a.ld_b);
+      a.a_mn = 1; a.b = data(xr); a.out = data(dw); a.rows = n; a.cols = (int)k; a.depth = (int)rows;
+      check(hyc_linear_act_tcgen05(&a, on.stream), "hyc_linear_act_tcgen05");
+    }
+  }
+  return {dx, dw, db};
+}
+
 void bind_forms(pybind11::module_& m) {
+  m.def("linear_act_forward", &linear_act_forward);
+  m.def("linear_act_backward", &linear_act_backward);
+  m.def("linear_status", [](int64_t device) {
+    c10::cuda::CUDAGuard guard((c10::DeviceIndex)device);
+    int status = 0;
+    check(hyc_linear_status(&status), "hyc_linear_status");
+    return status;
+  });
   m.def("softmax_relative_bias_forward", &softmax_relative_bias_forward);
   m.def("softmax_relative_bias_backward", &softmax_relative_bias_backward);
   m.def("qk_norm_rope_forward", &qk_norm_rope_forward);

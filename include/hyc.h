@@ -560,6 +560,32 @@ int hyc_softmax_relative_bias_fwd(const hyc_relative_bias* args, void* stream);
 size_t hyc_softmax_relative_bias_workspace_bytes(const hyc_relative_bias* args);
 int hyc_softmax_relative_bias_bwd(const hyc_relative_bias* args, float* dtable, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- products with bias, activation and residual in the epilogue ---------------------
+ *
+ * out[r, c] = act(pre[r, c]) + residual[r, c],  pre[r, c] = sum_k A[r, k] B[c, k] + bias[c], of bf16 or fp16 operands, fp32 inside, each
+ * result rounded once (act takes the unrounded sum; pre, optional, is what backward needs).
+ *   a: A[r, k] at a[r * ld_a + k], or with a_mn at a[k * ld_a + r]; b: B[c, k] at b[c * ld_b + k], or with b_mn at b[k * ld_b + c].  a_mn only
+ *   together with b_mn.  Forward of x [T, K] and W [N, K]: a = x, b = W.  dx = dpre W: a = dpre, b = W, b_mn, depth N.  dW = dpre^T x:
+ *   a = dpre, a_mn, b = x, b_mn, depth T.
+ *   rows: any number (a multiple of 8 with a_mn); cols a multiple of 8; depth a multiple of 8 unless a_mn (then any).  Row strides are
+ *   multiples of 8 elements, operands, residual, pre and out lie on 16 bytes; out and pre are contiguous.
+ * act: HYC_ACT_*; GELU is x Phi(x), GELU_TANH 0.5 x (1 + tanh(sqrt(2 / pi) (x + 0.044715 x^3))), SILU x / (1 + e^-x).
+ * dpre: dpre = dy * act'(pre) [rows, cols], rounded (HYC_ACT_NONE: neither read nor written), and, unless null, dbias [cols] = its column sums, of the
+ *   unrounded values, in a fixed order; dy with row stride ld_dy (0: one row for all); workspace for dbias.
+ * hyc_linear_status waits for the device and reads a word that stays 0 unless a bounded wait of these kernels gave up on it. */
+enum { HYC_ACT_NONE = 0, HYC_ACT_RELU = 1, HYC_ACT_GELU = 2, HYC_ACT_GELU_TANH = 3, HYC_ACT_SILU = 4 };
+typedef struct {
+  const void* a; const void* b; const void* bias; const void* residual;
+  void* pre; void* out;
+  int64_t ld_a, ld_b, ld_res, rows;
+  int cols, depth, a_mn, b_mn, type, act;
+} hyc_linear;
+int hyc_linear_act_tcgen05(const hyc_linear* args, void* stream);
+size_t hyc_linear_act_dpre_workspace_bytes(int cols);
+int hyc_linear_act_dpre(const void* dy, int64_t ld_dy, const void* pre, void* dpre, void* dbias, int64_t rows, int cols, int type, int act,
+                        void* workspace, size_t workspace_bytes, void* stream);
+int hyc_linear_status(int* host_status);
+
 #ifdef __cplusplus
 }
 #endif
