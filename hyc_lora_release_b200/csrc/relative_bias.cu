@@ -11,8 +11,8 @@
 // belong to one warp; longer ones (WIDE) to the warps of a block, or of a cluster of blocks, which exchange one pair (largest
 // element, sum) per warp and row.
 //
-// Forward: the bias depends on j - i alone and is constant beyond the last edge, so that a table of 2 L + 1 values in shared
-// memory (L = the last edge) serves every row of a head; pieces of a row that lie beyond take the constant.
+// Forward: the bias depends on j - i alone, so that one vector of (columns + rows) values in shared memory serves all rows of a block;
+// an element's bias is one load from it, eight columns apart from lane to lane and spread over the banks.
 //
 // Backward: the table's gradient needs the sums of ds along diagonals.  A warp takes consecutive rows, and from row to row the
 // running sum of each diagonal moves one column to the right: within a lane's V columns that is an operand of the addition, between
@@ -25,7 +25,8 @@
 namespace hyc {
 
 constexpr int kRbMaxSide = 128;          // buckets of one side
-constexpr int kRbNarrowWarps = 8;        // warps of a block whose warps have rows of their own
+constexpr int kRbNarrowWarps = 8;        // forward: warps of a block whose warps have rows of their own
+constexpr int kRbBwdWarps = 4;           // backward: the same
 constexpr int kRbMaxWarps = 16;          // warps of a block that share a row
 constexpr int kRbMaxCluster = 8;
 
@@ -39,6 +40,7 @@ struct RbParams {
   int rows_per, chunks;                  // rows of a warp (narrow: of a warp; wide: of a block or cluster), chunks of a head's rows
   int cluster;                           // blocks that share a row
   int table_type, mask_type, mask_vec;
+  int mask_staged;                       // values of the mask that a block keeps in shared memory, or 0
   int side, both, causal, buckets;
   float scale;
   int edges[kRbMaxSide];
@@ -65,21 +67,92 @@ __device__ __forceinline__ void st_piece(__half* p, const float (&f)[2]) { *rein
 __device__ __forceinline__ void st_piece(__nv_bfloat16* p, const float (&f)[2]) { *reinterpret_cast<uint32_t*>(p) = pack_bf16x2_rn(f[0], f[1]); }
 template <typename T> __device__ __forceinline__ void st_piece(T* p, const float (&f)[1]) { *p = from_f32<T>(f[0]); }
 
-__device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
+__device__ __forceinline__ float warp_max(float v) {      // (a NaN among the values is passed over)
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
 }
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-// e^v for v <= 0 (or NaN): two roundings and the two units in the last place of the instruction; below 2^-126 it is 0
-__device__ __forceinline__ float exp_neg(float v) {
+// Exponents are kept times log2(e), so that an exponential is one subtraction and one instruction (two units in the last place; below
+// 2^-126 it is 0).
+constexpr float kLog2e = 1.4426950408889634f;
+__device__ __forceinline__ float exp2_neg(float v) {
   float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v * 1.4426950408889634f));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
+}
+// a mask's value times log2(e): a finite one stays finite (the type's lowest value must not become -infinity)
+constexpr float kLowest = -3.402823466e38f;
+__device__ __forceinline__ float mask_log2e(float m) {
+  const float v = m * kLog2e;
+  return v == -INFINITY && m != -INFINITY ? kLowest : v;
+}
+
+// ---- two fp32 operations per instruction, over the V values of a piece
+__device__ __forceinline__ uint64_t two(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void halves(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+template <int V>
+__device__ __forceinline__ void fma_all(float (&x)[V], float s, const float (&b)[V]) {      // x = x s + b
+  if constexpr (V == 1) { x[0] = fmaf(x[0], s, b[0]); }
+  else {
+#pragma unroll
+    for (int e = 0; e < V; e += 2) {
+      uint64_t r;
+      asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(two(x[e], x[e + 1])), "l"(two(s, s)), "l"(two(b[e], b[e + 1])));
+      halves(r, x[e], x[e + 1]);
+    }
+  }
+}
+template <int V>
+__device__ __forceinline__ void add_all(float (&x)[V], const float (&b)[V]) {
+  if constexpr (V == 1) { x[0] += b[0]; }
+  else {
+#pragma unroll
+    for (int e = 0; e < V; e += 2) {
+      uint64_t r;
+      asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(two(x[e], x[e + 1])), "l"(two(b[e], b[e + 1])));
+      halves(r, x[e], x[e + 1]);
+    }
+  }
+}
+template <int V>
+__device__ __forceinline__ void add_one(float (&x)[V], float b) {
+  float v[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) v[e] = b;
+  add_all(x, v);
+}
+template <int V>
+__device__ __forceinline__ void mul_one(float (&x)[V], float b) {
+  if constexpr (V == 1) { x[0] *= b; }
+  else {
+#pragma unroll
+    for (int e = 0; e < V; e += 2) {
+      uint64_t r;
+      asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(two(x[e], x[e + 1])), "l"(two(b, b)));
+      halves(r, x[e], x[e + 1]);
+    }
+  }
+}
+template <int V>
+__device__ __forceinline__ void mul_all(float (&x)[V], const float (&b)[V]) {
+  if constexpr (V == 1) { x[0] *= b[0]; }
+  else {
+#pragma unroll
+    for (int e = 0; e < V; e += 2) {
+      uint64_t r;
+      asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(two(x[e], x[e + 1])), "l"(two(b[e], b[e + 1])));
+      halves(r, x[e], x[e + 1]);
+    }
+  }
 }
 
 // ---- exchange between the warps that share a row: every warp gives a pair and receives all of them combined.  `turn` alternates,
@@ -115,11 +188,11 @@ __device__ __forceinline__ float2 rb_exchange(RbExchange& ex, int turn, int warp
 __device__ __forceinline__ float2 join_softmax(float2 a, float2 b) {
   const float m = fmaxf(a.x, b.x);
   if (m == -INFINITY) return make_float2(m, a.y + b.y);
-  return make_float2(m, a.y * exp_neg(a.x - m) + b.y * exp_neg(b.x - m));
+  return make_float2(m, a.y * exp2_neg(a.x - m) + b.y * exp2_neg(b.x - m));
 }
 
-// the bias table, spread so that lanes eight columns apart meet in no bank
-__device__ __forceinline__ int lut_at(int x) { return x + (x >> 3); }
+// the bias table, spread for lanes eight columns apart so that they meet in no bank
+template <int V> __device__ __forceinline__ int lut_at(int x) { return V == 8 ? x + (x >> 3) : x; }
 
 __device__ __forceinline__ int rb_bucket(const int* edges, int side, int distance) {      // number of edges <= distance, less one
   int lo = 0, hi = side;                                                                // edges[lo] <= distance < edges[hi]
@@ -130,109 +203,161 @@ __device__ __forceinline__ int rb_bucket(const int* edges, int side, int distanc
   return lo;
 }
 
+// columns of row i that count
+__device__ __forceinline__ int rb_end(const RbParams& p, int i) {
+  const int q = i + p.q_offset;
+  return p.causal ? max(0, min(q + 1, p.cols)) : p.cols;
+}
+
 template <typename T, int V, int NV, bool WIDE>
-__global__ void __launch_bounds__(WIDE ? 32 * kRbMaxWarps : 32 * kRbNarrowWarps)
+__global__ void __launch_bounds__(WIDE ? 32 * kRbMaxWarps : 32 * kRbNarrowWarps, WIDE ? 1 : 2)
 relbias_fwd_kernel(const __grid_constant__ RbParams p) {
-  extern __shared__ float s_lut[];
+  extern __shared__ __align__(16) float s_mem[];
   __shared__ int s_edges[kRbMaxSide];
+  __shared__ float s_table[2 * kRbMaxSide];
   __shared__ RbExchange s_ex;
   constexpr int SPAN = 32 * V * NV;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), warps = blockDim.x >> 5;
   const int rank = WIDE ? (int)(blockIdx.x % (unsigned)p.cluster) : 0;
+  float *s_mask = s_mem, *s_lut = s_mem + p.mask_staged;      // a mask that all rows share, the block's columns; the bias
   const uint32_t unit = blockIdx.x / (unsigned)p.cluster;
-  const int bh = (int)(unit / (uint32_t)p.chunks), chunk = (int)(unit - (uint32_t)bh * (uint32_t)p.chunks);
+  const int bh = (int)(unit / (uint32_t)p.chunks), chunk = p.chunks - 1 - (int)(unit - (uint32_t)bh * (uint32_t)p.chunks);      // (causal: long rows first)
   const int b = bh / p.heads, h = bh - b * p.heads;
-  const int step = WIDE ? 1 : kRbNarrowWarps;
-  const int first = chunk * p.rows_per * step + (WIDE ? 0 : warp);
-  const int last = min((chunk + 1) * p.rows_per * step, p.n);
-  const int far = p.edges[p.side - 1], ahead = p.both ? far : 0;      // distances are told apart from -far to ahead
+  const int first = (WIDE ? chunk : chunk * kRbNarrowWarps + warp) * p.rows_per, last = min(first + p.rows_per, p.n);
+  const int block_rows = WIDE ? p.rows_per : kRbNarrowWarps * p.rows_per;
+  const int q_last = min((chunk + 1) * block_rows, p.n) - 1 + p.q_offset;      // of the block's rows
+  const int block_c0 = WIDE ? rank * warps * SPAN : 0;
+  const int c0 = WIDE ? block_c0 + warp * SPAN : 0;
+  const int64_t map = (int64_t)bh * p.n;
+  // (at the lane's first column of the row to be read, of the row to be written)
+  const int cl = c0 + lane * V;
+  const T* src = reinterpret_cast<const T*>(p.x) + (map + first) * p.cols + cl;
+  T* dst = reinterpret_cast<T*>(p.out) + (map + first) * p.cols + cl;
   for (int i = threadIdx.x; i < p.side; i += blockDim.x) s_edges[i] = p.edges[i];
   pdl_wait();
+  Piece<T, V> raw[NV];                  // the row to come
+  if (first < last) {
+    const int end = rb_end(p, first);
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+      if (cl + k * 32 * V < end) ld_piece(src + k * 32 * V, raw[k]);
+  }
+  for (int i = threadIdx.x; i < p.buckets; i += blockDim.x) s_table[i] = ld_any(p.table, (int64_t)i * p.heads + h, p.table_type) * kLog2e;
+  if (p.mask_staged) {
+    const int64_t at = b * p.mask_b + h * p.mask_h;
+    for (int i = threadIdx.x; i < p.mask_staged && block_c0 + i < p.cols; i += blockDim.x) s_mask[i] = mask_log2e(ld_any(p.mask, at + block_c0 + i, p.mask_type));
+  }
   __syncthreads();
-  for (int i = threadIdx.x; i <= far + ahead; i += blockDim.x) {
-    const int d = i - far;
-    const int k = rb_bucket(s_edges, p.side, d < 0 ? -d : (p.both ? d : 0)) + (p.both && d > 0 ? p.side : 0);
-    s_lut[lut_at(i)] = ld_any(p.table, (int64_t)k * p.heads + h, p.table_type);
+  // the bias of every distance that the block meets, from its first column and last row on
+  const int far = p.edges[p.side - 1], width = WIDE ? warps * SPAN : SPAN;
+  for (int i = threadIdx.x; i < min(width, p.cols - block_c0) + block_rows; i += blockDim.x) {
+    const int d = block_c0 - q_last + i;
+    const int r = d < 0 ? -d : (p.both ? d : 0);
+    const int k = r >= far ? p.side - 1 : rb_bucket(s_edges, p.side, r);
+    s_lut[lut_at<V>(i)] = s_table[k + (p.both && d > 0 ? p.side : 0)];
   }
   __syncthreads();
   if (WIDE && p.cluster > 1) rb_cluster_sync();      // the other blocks have started: their shared memory may be written
-  const float bias_behind = s_lut[0], bias_ahead = s_lut[lut_at(far + ahead)];
-  const int c0 = WIDE ? (rank * warps + warp) * SPAN : 0;
-  const int64_t map = (int64_t)bh * p.n;
-  const T* x = reinterpret_cast<const T*>(p.x) + map * p.cols;
-  T* out = reinterpret_cast<T*>(p.out) + map * p.cols;
+  const float scale = p.scale * kLog2e;
+  const float* my_mask = s_mask + (cl - block_c0);
   int turn = 0;
-  for (int i = first; i < last; i += step, turn ^= 1) {
-    const int q = i + p.q_offset;
-    const int end = p.causal ? (q < -1 ? 0 : (q + 1 < p.cols ? q + 1 : p.cols)) : p.cols;      // columns that count
-    const T* row = x + (int64_t)i * p.cols;
-    Piece<T, V> raw[NV];
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int c = c0 + k * 32 * V + lane * V;
-      if (c < end) ld_piece(row + c, raw[k]);
-    }
+  for (int i = first; i < last; ++i, turn ^= 1, dst += p.cols) {
+    const int q = i + p.q_offset, end = rb_end(p, i), end_next = i + 1 < last ? rb_end(p, i + 1) : 0;
+    // the lane's columns in the bias table: eight apart, so that the shift within eight is the same for all of them
+    const int shift = q_last - q, within = V == 8 ? shift & 7 : 0;
+    const float* lut = V == 8 ? s_lut + 9 * ((cl - block_c0) / 8 + (shift >> 3)) : s_lut + (cl - block_c0 + shift);
+    src += p.cols;
     float f[NV][V], m = -INFINITY;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int cb = c0 + k * 32 * V, c = cb + lane * V;
-      if (cb >= end) {                   // (the whole warp)
-#pragma unroll
-        for (int e = 0; e < V; ++e) f[k][e] = -INFINITY;
-        continue;
-      }
+      piece_f32(raw[k], f[k]);
+      if (c < end_next) ld_piece(src + k * 32 * V, raw[k]);      // (its place is free: the next row's is on its way from here on)
+      if (cb >= end) continue;           // (the whole warp)
       float bias[V];
-      const int dmin = cb - q, dmax = cb + 32 * V - 1 - q;
-      if (dmax <= -far || dmin >= ahead) {
-        const float v = dmax <= -far ? bias_behind : bias_ahead;
 #pragma unroll
-        for (int e = 0; e < V; ++e) bias[e] = v;
-      } else {
+      for (int e = 0; e < V; ++e) bias[e] = V == 8 ? lut[k * 32 * 9 + lut_at<V>(within + e)] : lut[k * 32 * V + e];
+      fma_all(f[k], scale, bias);
+    }
+    if (p.mask_staged) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) bias[e] = s_lut[lut_at(min(max(c + e - q, -far), ahead) + far)];
-      }
-      if (p.mask != nullptr && c < end) {
-        const int64_t at = b * p.mask_b + h * p.mask_h + (int64_t)i * p.mask_row + c;
-        if (V == 8 && p.mask_vec) {
-          float mk[8];
-          ld_any8(p.mask, at, p.mask_type, mk);
-#pragma unroll
-          for (int e = 0; e < V; ++e) bias[e] += mk[e & 7];
+      for (int k = 0; k < NV; ++k) {
+        // (behind the row's last column: whatever lies there, the columns do not count)
+        float mk[V];
+        if constexpr (V == 8) {
+          *reinterpret_cast<float4*>(mk) = *reinterpret_cast<const float4*>(my_mask + k * 32 * V);
+          *reinterpret_cast<float4*>(mk + 4) = *reinterpret_cast<const float4*>(my_mask + k * 32 * V + 4);
         } else {
 #pragma unroll
-          for (int e = 0; e < V; ++e) bias[e] += ld_any(p.mask, at + e, p.mask_type);
+          for (int e = 0; e < V; ++e) mk[e] = my_mask[k * 32 * V + e];
         }
+        add_all(f[k], mk);
       }
-      if (c < end) piece_f32(raw[k], f[k]);
+    } else if (p.mask != nullptr) {
+      const int64_t at = b * p.mask_b + h * p.mask_h + (int64_t)i * p.mask_row + cl;
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        f[k][e] = c + e < end ? fmaf(f[k][e], p.scale, bias[e]) : -INFINITY;
-        m = fmaxf(m, f[k][e]);
+      for (int k = 0; k < NV; ++k) {
+        if (cl + k * 32 * V >= end) continue;
+        float mk[V];
+        if constexpr (V == 8) {
+          if (p.mask_vec) {
+            ld_any8(p.mask, at + k * 32 * V, p.mask_type, mk);
+          } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) mk[e] = ld_any(p.mask, at + k * 32 * V + e, p.mask_type);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; ++e) mk[e] = ld_any(p.mask, at + k * 32 * V + e, p.mask_type);
+        }
+#pragma unroll
+        for (int e = 0; e < V; ++e) mk[e] = mask_log2e(mk[e]);
+        add_all(f[k], mk);
       }
     }
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int cb = c0 + k * 32 * V, c = cb + lane * V;
+      if (cb + 32 * V > end) {           // (else all of the warp's columns count)
+#pragma unroll
+        for (int e = 0; e < V; ++e) f[k][e] = c + e < end ? f[k][e] : -INFINITY;
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) m = fmaxf(m, f[k][e]);
+    }
     m = warp_max(m);
-    const float mm = m == -INFINITY ? 0.f : m;      // nothing counts: e^-inf = 0 everywhere
-    float sum = 0.f;
+    const float mm = m == -INFINITY ? 0.f : m;      // nothing counts: 2^-inf = 0 everywhere
+    float sums[V], sum = 0.f;
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
+    for (int e = 0; e < V; ++e) sums[e] = 0.f;
 #pragma unroll
-      for (int e = 0; e < V; ++e) { f[k][e] = exp_neg(f[k][e] - mm); sum += f[k][e]; }
+    for (int k = 0; k < NV; ++k) {
+      if (c0 + k * 32 * V >= end) continue;
+      add_one(f[k], -mm);
+#pragma unroll
+      for (int e = 0; e < V; ++e) f[k][e] = exp2_neg(f[k][e]);
+      add_all(sums, f[k]);
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) sum += sums[e];
     sum = warp_sum(sum);
     float factor;
     if (WIDE) {
       const float2 all = rb_exchange(s_ex, turn, warps, p.cluster, rank, make_float2(m, sum), join_softmax);
-      factor = (m == -INFINITY ? 1.f : exp_neg(m - all.x)) / all.y;
+      factor = (m == -INFINITY ? 1.f : exp2_neg(m - all.x)) / all.y;
       if (all.y == 0.f) factor = 0.f;
     } else {
-      factor = sum == 0.f ? 0.f : 1.f / sum;        // a row that nothing is visible to: zeros
+      factor = sum == 0.f ? 0.f : __fdividef(1.f, sum);        // a row that nothing is visible to: zeros
     }
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int c = c0 + k * 32 * V + lane * V;
-      if (c >= p.cols) continue;
+      const int cb = c0 + k * 32 * V, c = cb + lane * V;
+      mul_one(f[k], factor);
+      if (cb + 32 * V > end) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) f[k][e] = c + e < end ? f[k][e] * factor : 0.f;      // (zero in a row that became NaN, too)
-      st_piece(out + (int64_t)i * p.cols + c, f[k]);
+        for (int e = 0; e < V; ++e) f[k][e] = c + e < end ? f[k][e] : 0.f;      // (zero in a row that became NaN, too)
+      }
+      if (c < p.cols) st_piece(dst + k * 32 * V, f[k]);
     }
   }
 }
@@ -249,8 +374,11 @@ __device__ __forceinline__ void rb_range(const RbParams& p, const int* edges, in
   }
 }
 
+// Blocks per SM that the registers of a narrow kernel are cut for: 3 (168 registers) where a lane has 64 elements, or 32 that take a
+// register each
+template <typename T, int V, int NV> constexpr int kRbBwdBlocks = V * NV == 64 || (V * NV == 32 && (V == 1 || sizeof(T) == 4)) ? 3 : 4;
 template <typename T, int V, int NV, bool WIDE>
-__global__ void __launch_bounds__(WIDE ? 32 * kRbMaxWarps : 32 * kRbNarrowWarps)
+__global__ void __launch_bounds__(WIDE ? 32 * kRbMaxWarps : 32 * kRbBwdWarps, WIDE ? 1 : kRbBwdBlocks<T, V, NV>)
 relbias_bwd_kernel(const __grid_constant__ RbParams p) {
   extern __shared__ float s_diag_all[];
   __shared__ int s_edges[kRbMaxSide];
@@ -263,71 +391,89 @@ relbias_bwd_kernel(const __grid_constant__ RbParams p) {
   pdl_wait();
   if (WIDE && p.cluster > 1) rb_cluster_sync();      // the other blocks have started: their shared memory may be written
   // a unit: `rows_per` consecutive rows of one map, for a warp or for the warps that share a row
-  const int64_t unit = WIDE ? blockIdx.x / (unsigned)p.cluster : (int64_t)blockIdx.x * kRbNarrowWarps + warp;
-  const int bh = (int)(unit / p.chunks), chunk = (int)(unit - (int64_t)bh * p.chunks);
-  const int first = chunk * p.rows_per, last = min(first + p.rows_per, p.n) - 1;
+  const int64_t unit = WIDE ? blockIdx.x / (unsigned)p.cluster : (int64_t)blockIdx.x * kRbBwdWarps + warp;
   if (!WIDE && unit >= p.units) return;
+  const int bh = (int)(unit / p.chunks), chunk = p.chunks - 1 - (int)(unit - (int64_t)bh * p.chunks);      // (causal: long rows first)
+  const int first = chunk * p.rows_per, last = min(first + p.rows_per, p.n) - 1;
   float* s_diag = s_diag_all + warp * (SPAN + p.rows_per);
   const int c0 = WIDE ? (rank * warps + warp) * SPAN : 0;
   const int64_t map = (int64_t)bh * p.n;
-  const T *a = reinterpret_cast<const T*>(p.x) + map * p.cols, *g = reinterpret_cast<const T*>(p.grad) + map * p.cols;
-  T* out = reinterpret_cast<T*>(p.out) + map * p.cols;
+  const int cl = c0 + lane * V;
+  const T *a = reinterpret_cast<const T*>(p.x) + (map + first) * p.cols + cl, *g = reinterpret_cast<const T*>(p.grad) + (map + first) * p.cols + cl;
+  T* dst = reinterpret_cast<T*>(p.out) + (map + first) * p.cols + cl;
+  Piece<T, V> ra[NV], rg[NV];           // the row to come
+  {
+    const int end = rb_end(p, first);
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+      if (cl + k * 32 * V < end) { ld_piece(a + k * 32 * V, ra[k]); ld_piece(g + k * 32 * V, rg[k]); }
+  }
   float acc[NV][V];
 #pragma unroll
   for (int k = 0; k < NV; ++k)
 #pragma unroll
     for (int e = 0; e < V; ++e) acc[k][e] = 0.f;
   int turn = 0;
-  for (int i = first; i <= last; ++i, turn ^= 1) {
-    const int q = i + p.q_offset;
-    const int end = p.causal ? (q < -1 ? 0 : (q + 1 < p.cols ? q + 1 : p.cols)) : p.cols;
-    float ds[NV][V], dot = 0.f;
-    Piece<T, V> ra[NV], rg[NV];
+  for (int i = first; i <= last; ++i, turn ^= 1, dst += p.cols) {
+    const int end = rb_end(p, i);
+    const int end_next = i < last ? rb_end(p, i + 1) : 0;
+    a += p.cols;
+    g += p.cols;
+    float dots[V], dot = 0.f;
+#pragma unroll
+    for (int e = 0; e < V; ++e) dots[e] = 0.f;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int c = c0 + k * 32 * V + lane * V;
-      if (c < end) {
-        ld_piece(a + (int64_t)i * p.cols + c, ra[k]);
-        ld_piece(g + (int64_t)i * p.cols + c, rg[k]);
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int c = c0 + k * 32 * V + lane * V;
-      if (c >= end) continue;
+      const int cb = c0 + k * 32 * V, c = cb + lane * V;
+      if (cb >= end) continue;           // (the whole warp, as below)
       float fa[V], fg[V];
       piece_f32(ra[k], fa);
       piece_f32(rg[k], fg);
+      if (cb + 32 * V <= end) {
+        mul_all(fa, fg);
+        add_all(dots, fa);
+      } else {
 #pragma unroll
-      for (int e = 0; e < V; ++e)
-        if (c + e < end) dot = fmaf(fa[e], fg[e], dot);
-    }
-    dot = warp_sum(dot);
-    if (WIDE) dot = rb_exchange(s_ex, turn, warps, p.cluster, rank, make_float2(dot, 0.f), [](float2 u, float2 v) { return make_float2(u.x + v.x, 0.f); }).x;
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int c = c0 + k * 32 * V + lane * V;
-      float fa[V], fg[V];
-      if (c < end) { piece_f32(ra[k], fa); piece_f32(rg[k], fg); }
-#pragma unroll
-      for (int e = 0; e < V; ++e) ds[k][e] = c + e < end ? fa[e] * (fg[e] - dot) : 0.f;
-      if (c < p.cols) {
-        float o[V];
-#pragma unroll
-        for (int e = 0; e < V; ++e) o[e] = ds[k][e] * p.scale;
-        st_piece(out + (int64_t)i * p.cols + c, o);
+        for (int e = 0; e < V; ++e)
+          if (c + e < end) dots[e] = fmaf(fa[e], fg[e], dots[e]);
       }
     }
-    // the diagonals' running sums one column to the right, this row's share added
+#pragma unroll
+    for (int e = 0; e < V; ++e) dot += dots[e];
+    dot = warp_sum(dot);
+    if (WIDE) dot = rb_exchange(s_ex, turn, warps, p.cluster, rank, make_float2(dot, 0.f), [](float2 u, float2 v) { return make_float2(u.x + v.x, 0.f); }).x;
+    // the gradient, and the diagonals' running sums: one column to the right, this row's share added
     float left = 0.f;                    // lane 0: what leaves the piece of columns before
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
+      const int cb = c0 + k * 32 * V, c = cb + lane * V;
+      float ds[V], o[V], fg[V];
+      piece_f32(ra[k], ds);
+      piece_f32(rg[k], fg);
+      if (c < end_next) { ld_piece(a + k * 32 * V, ra[k]); ld_piece(g + k * 32 * V, rg[k]); }      // (the places are free: the next row's are on their way)
+      if (cb >= end) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) { ds[e] = 0.f; o[e] = 0.f; }
+        if (c < p.cols) st_piece(dst + k * 32 * V, o);
+        if (p.causal) { left = 0.f; continue; }      // columns that no row so far has seen: no sums either
+      } else {
+        add_one(fg, -dot);
+        mul_all(ds, fg);
+        if (cb + 32 * V > end) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) ds[e] = c + e < end ? ds[e] : 0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < V; ++e) o[e] = ds[e];
+        mul_one(o, p.scale);
+        if (c < p.cols) st_piece(dst + k * 32 * V, o);
+      }
       const float moved = __shfl_sync(0xffffffffu, acc[k][V - 1], (lane + 31) & 31);
       const float carry = lane == 0 ? left : moved;
       left = moved;
 #pragma unroll
-      for (int e = V - 1; e > 0; --e) acc[k][e] = acc[k][e - 1] + ds[k][e];
-      acc[k][0] = carry + ds[k][0];
+      for (int e = V - 1; e > 0; --e) acc[k][e] = acc[k][e - 1] + ds[e];
+      acc[k][0] = carry + ds[0];
     }
     if (lane == 0 && i > first) s_diag[SPAN + last - i] = left;
   }
@@ -339,20 +485,24 @@ relbias_bwd_kernel(const __grid_constant__ RbParams p) {
   // s_diag[x] is the sum of the diagonal at distance x + dmin
   const int dmin = c0 - last - p.q_offset, dmax = dmin + SPAN - 1 + (last - first);
   float* part = p.part + ((WIDE ? unit * p.cluster * warps + rank * warps + warp : unit)) * p.buckets;
-  float mine = 0.f;
-  for (int k = 0; k < p.buckets; ++k) {
-    int from, to;
-    rb_range(p, s_edges, k, from, to);
+  // short ranges by a lane each, long ones by the warp
+  for (int k0 = 0; k0 < p.buckets; k0 += 32) {
+    const int k = k0 + lane;
+    int from = 1, to = 0;
+    if (k < p.buckets) rb_range(p, s_edges, k, from, to);
     from = max(from, dmin); to = min(to, dmax);
+    const bool wide_range = to - from >= 48;
     float sum = 0.f;
-    if (from <= to) {
-      for (int d = from + lane; d <= to; d += 32) sum += s_diag[d - dmin];
-      sum = warp_sum(sum);
+    if (!wide_range)
+      for (int d = from; d <= to; ++d) sum += s_diag[d - dmin];
+    for (unsigned left = __ballot_sync(0xffffffffu, wide_range); left != 0u; left &= left - 1u) {
+      const int l = __ffs(left) - 1, lo = __shfl_sync(0xffffffffu, from, l), hi = __shfl_sync(0xffffffffu, to, l);
+      float v = 0.f;
+      for (int d = lo + lane; d <= hi; d += 32) v += s_diag[d - dmin];
+      v = warp_sum(v);
+      if (lane == l) sum = v;
     }
-    if ((k & 31) == lane) mine = sum;
-    if ((k & 31) == 31 || k == p.buckets - 1) {
-      if ((k & ~31) + lane < p.buckets) part[(k & ~31) + lane] = mine;
-    }
+    if (k < p.buckets) part[k] = sum;
   }
 }
 
@@ -363,11 +513,14 @@ relbias_table_kernel(const float* __restrict__ part, int batch, int heads, int p
   pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, h = (int)blockIdx.x, k = (int)blockIdx.y * 32 + lane;
   double sum = 0.0;
-  if (k < buckets)
-    for (int b = 0; b < batch; ++b) {
-      const float* src = part + ((int64_t)(b * heads + h) * per_map) * buckets + k;
-      for (int u = warp; u < per_map; u += 32) sum += (double)src[(int64_t)u * buckets];
+  const uint32_t units = (uint32_t)batch * (uint32_t)per_map;
+  if (k < buckets) {
+#pragma unroll 4
+    for (uint32_t u = warp; u < units; u += 32) {
+      const uint32_t b = u / (uint32_t)per_map;
+      sum += (double)part[((int64_t)(b * heads + h) * per_map + (u - b * per_map)) * buckets + k];
     }
+  }
   s_sum[warp][lane] = sum;
   __syncthreads();
   sum = s_sum[lane][warp];
@@ -397,7 +550,9 @@ static int rb_check(const hyc_relative_bias* a, bool backward) {
   return HYC_OK;
 }
 
-// How a map is cut: V adjacent elements per access, accesses per lane, warps (and blocks of a cluster) of a row
+// How a map is cut: V adjacent elements per access, accesses per lane, warps (and blocks of a cluster) of a row.  A warp whose lanes have
+// more elements spends less on what every row costs (reductions, addresses) and has fewer companions to wait for; what limits it is
+// registers: 64 elements of 16-bit octets, 32 of the rest.
 struct RbPlan { int v, nv, warps, cluster; bool wide; };
 static RbPlan rb_plan(const hyc_relative_bias* a, bool backward) {
   RbPlan r;
@@ -407,31 +562,35 @@ static RbPlan rb_plan(const hyc_relative_bias* a, bool backward) {
     return a->cols % v == 0 && aligned(a->x, bytes) && aligned(a->out, bytes) && (!backward || aligned(a->grad, bytes));
   };
   r.v = fits(8) ? 8 : fits(2) ? 2 : 1;
-  const int64_t rows = a->batch * a->heads * a->n, cols = a->cols;
+  const int64_t cols = a->cols, rows = a->batch * a->heads * a->n;
   r.cluster = 1;
-  if (cols <= 1024) {
-    r.wide = false;
-    r.warps = kRbNarrowWarps;
-    r.nv = (cols <= 256 ? 256 : cols <= 512 && r.v == 8 ? 512 : 1024) / (32 * r.v);
-    return r;
+  r.warps = backward ? kRbBwdWarps : kRbNarrowWarps;
+  // few rows: several warps each, for what a row takes
+  const bool few = cols > 512 && rows < (int64_t)num_sms() * 8;
+  int span = 256;
+  while (span < cols && span < (e == 2 && r.v == 8 ? 2048 : 1024)) span *= 2;
+  r.wide = few || cols > span;
+  if (r.wide) {
+    span = few && cols <= 256 * kRbMaxWarps ? 256 : 1024;
+    while (cols > (int64_t)r.cluster * kRbMaxWarps * span) r.cluster *= 2;
+    r.warps = (int)((cols + (int64_t)r.cluster * span - 1) / ((int64_t)r.cluster * span));
   }
-  // few rows: as many warps as a block may have; many: as few as can hold a row, for fewer exchanges
-  r.wide = true;
-  int span = 1024;
-  if (cols <= 256 * kRbMaxWarps && rows * ((cols + 1023) / 1024) < (int64_t)num_sms() * 16) span = 256;
-  while (cols > (int64_t)r.cluster * kRbMaxWarps * span) r.cluster *= 2;
-  r.warps = (int)((cols + (int64_t)r.cluster * span - 1) / ((int64_t)r.cluster * span));
   r.nv = span / (32 * r.v);
   return r;
 }
-// rows of a unit, so that there are a few times as many units as can be resident
-static int rb_rows_per(const RbPlan& r, int64_t rows, int n, int most) {
-  const int64_t resident = (int64_t)num_sms() * 32 / (r.wide ? r.warps * r.cluster : 1);
-  int64_t per = rows / (resident < 1 ? 1 : 2 * resident);
-  per = per < 1 ? 1 : per > most ? most : per;
-  return (int)(per > n ? n : per);
+// Rows of a unit (narrow: a warp, wide: the warps that share a row): what a unit takes to start and end, in rows, against units that do not
+// fill the last wave.  warps: units of a block of forward; slots: blocks (backward: units) that are resident at once; causal rows are unlike, long ones come first, so the waves overlap.
+static int rb_rows_per(int64_t maps, int n, int warps, int64_t slots, float fixed, bool causal) {
+  int best = 1;
+  float best_cost = 1e30f;
+  for (int per = 1; per <= 32; ++per) {
+    const int64_t units = maps * ((n + per * warps - 1) / (per * warps));
+    const float waves = (float)units / (float)slots, whole = (float)((units + slots - 1) / slots);
+    const float cost = (causal && waves > 1.f ? waves + 0.5f : whole) * ((float)per + fixed);
+    if (cost < best_cost * 0.999f) { best_cost = cost; best = per; }
+  }
+  return best < n ? best : n;
 }
-constexpr int kRbRowsFwd = 16, kRbRowsBwd = 32;
 
 static void rb_fill(RbParams& p, const hyc_relative_bias* a, const RbPlan& r) {
   p.x = a->x; p.grad = a->grad; p.table = a->table; p.mask = a->mask; p.out = a->out; p.part = nullptr;
@@ -442,6 +601,7 @@ static void rb_fill(RbParams& p, const hyc_relative_bias* a, const RbPlan& r) {
   p.mask_vec = a->mask != nullptr && aligned(a->mask, 16) && ((a->mask_b | a->mask_h | a->mask_row) & 7) == 0;
   p.side = a->side; p.both = a->both != 0; p.causal = a->causal != 0; p.buckets = a->both ? 2 * a->side : a->side;
   p.scale = a->scale;
+  p.mask_staged = 0;
   for (int i = 0; i < a->side; ++i) p.edges[i] = a->host_edges[i];
 }
 
@@ -471,37 +631,39 @@ static int rb_launch(K kern, const RbPlan& r, int64_t blocks, size_t smem, const
   return HYC_OK;
 }
 
-// f(element, V, NV, WIDE) for the plan's kernel
+// f(element, V, NV, WIDE) for the plan's kernel: narrow spans of 256 to 1024 columns, 2048 of 16-bit octets; wide ones of 256 and 1024
 template <typename F>
 static int rb_by_plan(int type, const RbPlan& r, F&& f) {
   auto by_shape = [&](auto elem) -> int {
-    auto wide = [&](auto v, auto nv) -> int {
-      if (r.wide) return f(elem, v, nv, std::true_type());
-      return f(elem, v, nv, std::false_type());
+    auto span = [&](auto v) -> int {
+      constexpr int V = decltype(v)::value;
+      auto of = [&](auto nv) -> int {
+        if constexpr (decltype(nv)::value * V == 16) return f(elem, v, nv, std::false_type());
+        else if constexpr (decltype(nv)::value * V == 64) return f(elem, v, nv, std::false_type());
+        else return r.wide ? f(elem, v, nv, std::true_type()) : f(elem, v, nv, std::false_type());
+      };
+      if (r.nv == 8 / V) return of(std::integral_constant<int, 8 / V>());
+      if (r.nv == 16 / V) return of(std::integral_constant<int, 16 / V>());
+      if constexpr (V == 8 && sizeof(elem) == 2)
+        if (r.nv == 64 / V) return of(std::integral_constant<int, 64 / V>());
+      return of(std::integral_constant<int, 32 / V>());
     };
-    using std::integral_constant;
-    if (r.v == 8) {
-      if (r.nv == 1) return wide(integral_constant<int, 8>(), integral_constant<int, 1>());
-      if (r.nv == 2) return f(elem, integral_constant<int, 8>(), integral_constant<int, 2>(), std::false_type());
-      return wide(integral_constant<int, 8>(), integral_constant<int, 4>());
-    }
-    if (r.v == 2) {
-      if (r.nv == 4) return wide(integral_constant<int, 2>(), integral_constant<int, 4>());
-      return wide(integral_constant<int, 2>(), integral_constant<int, 16>());
-    }
-    if (r.nv == 8) return wide(integral_constant<int, 1>(), integral_constant<int, 8>());
-    return wide(integral_constant<int, 1>(), integral_constant<int, 32>());
+    if (r.v == 8) return span(std::integral_constant<int, 8>());
+    if (r.v == 2) return span(std::integral_constant<int, 2>());
+    return span(std::integral_constant<int, 1>());
   };
   if (type == HYC_F32) return by_shape(float());
   if (type == HYC_F16) return by_shape(__half());
   return by_shape(__nv_bfloat16());
 }
 
-// backward: rows of a unit and the warps' sums that the workspace holds
+// backward: rows of a unit and the warps' sums that the workspace holds (the same for a query and for a launch: nothing here asks the runtime)
 struct RbUnits { int rows_per, chunks; int64_t units, sums; };
 static RbUnits rb_units(const hyc_relative_bias* a, const RbPlan& r) {
   RbUnits u;
-  u.rows_per = rb_rows_per(r, a->batch * a->heads * a->n, (int)a->n, kRbRowsBwd);
+  const int64_t warps = r.v * r.nv == 64 || (r.v * r.nv == 32 && (r.v == 1 || a->type == HYC_F32)) ? 12 : 16;      // resident per SM: kRbBwdBlocks
+  const int64_t slots = (int64_t)num_sms() * warps / (r.wide ? r.warps * r.cluster : 1);
+  u.rows_per = rb_rows_per(a->batch * a->heads, (int)a->n, 1, slots < 1 ? 1 : slots, 6.f, a->causal != 0);
   u.chunks = (int)((a->n + u.rows_per - 1) / u.rows_per);
   u.units = a->batch * a->heads * u.chunks;
   u.sums = u.units * (r.wide ? r.warps * r.cluster : 1);
@@ -518,14 +680,19 @@ extern "C" HYC_API int hyc_softmax_relative_bias_fwd(const hyc_relative_bias* a,
   const RbPlan r = rb_plan(a, false);
   RbParams p;
   rb_fill(p, a, r);
-  p.rows_per = rb_rows_per(r, a->batch * a->heads * a->n, (int)a->n, kRbRowsFwd);
-  const int step = p.rows_per * (r.wide ? 1 : kRbNarrowWarps);
-  p.chunks = (int)((a->n + step - 1) / step);
-  const int far = p.edges[p.side - 1], values = far + (p.both ? far : 0) + 1;
-  const size_t smem = (size_t)(values + values / 8 + 1) * sizeof(float);
+  const int width = 32 * r.v * r.nv * (r.wide ? r.warps : 1);      // columns of a block
+  p.mask_staged = a->mask != nullptr && (a->mask_row == 0 || a->n == 1) ? width : 0;
   return rb_by_plan(a->type, r, [&](auto elem, auto v, auto nv, auto wide) -> int {
-    return rb_launch(relbias_fwd_kernel<decltype(elem), decltype(v)::value, decltype(nv)::value, decltype(wide)::value>, r,
-                     a->batch * a->heads * p.chunks * r.cluster, smem, p, (cudaStream_t)stream);
+    auto kern = relbias_fwd_kernel<decltype(elem), decltype(v)::value, decltype(nv)::value, decltype(wide)::value>;
+    auto bytes = [&](int rows) { return (size_t)(p.mask_staged + (width + rows) * 9 / 8 + 2) * sizeof(float); };
+    const int block_warps = r.wide ? 1 : kRbNarrowWarps;      // warps with rows of their own
+    const int resident = bytes(32 * block_warps) > 32768 ? 1 : resident_blocks(kern, 32 * r.warps, bytes(32 * block_warps), 1);
+    const int64_t slots = (int64_t)num_sms() * resident / r.cluster;
+    p.rows_per = rb_rows_per(a->batch * a->heads, (int)a->n, block_warps, slots < 1 ? 1 : slots, 3.f, a->causal != 0);
+    const int rows = p.rows_per * block_warps;      // of a block
+    p.chunks = (int)((a->n + rows - 1) / rows);
+    const size_t smem = bytes(rows);
+    return rb_launch(kern, r, a->batch * a->heads * p.chunks * r.cluster, smem, p, (cudaStream_t)stream);
   });
 }
 
@@ -550,7 +717,7 @@ extern "C" HYC_API int hyc_softmax_relative_bias_bwd(const hyc_relative_bias* a,
     rb_fill(p, a, r);
     p.part = (float*)workspace;
     p.rows_per = u.rows_per; p.chunks = u.chunks; p.units = u.units;
-    const int64_t blocks = r.wide ? u.units * r.cluster : (u.units + kRbNarrowWarps - 1) / kRbNarrowWarps;
+    const int64_t blocks = r.wide ? u.units * r.cluster : (u.units + kRbBwdWarps - 1) / kRbBwdWarps;
     const size_t smem = (size_t)r.warps * (size_t)(32 * r.v * r.nv + u.rows_per) * sizeof(float);
     const int rl = rb_by_plan(a->type, r, [&](auto elem, auto v, auto nv, auto wide) -> int {
       return rb_launch(relbias_bwd_kernel<decltype(elem), decltype(v)::value, decltype(nv)::value, decltype(wide)::value>, r, blocks, smem, p,
