@@ -210,7 +210,7 @@ __device__ __forceinline__ int rb_end(const RbParams& p, int i) {
 }
 
 template <typename T, int V, int NV, bool WIDE>
-__global__ void __launch_bounds__(WIDE ? 32 * kRbMaxWarps : 32 * kRbNarrowWarps, WIDE ? 1 : 2)
+__global__ void __launch_bounds__(WIDE ? 32 * kRbMaxWarps : 32 * kRbNarrowWarps, WIDE ? 1 : V * NV <= 8 ? 5 : V * NV <= 16 ? 4 : 2)
 relbias_fwd_kernel(const __grid_constant__ RbParams p) {
   extern __shared__ __align__(16) float s_mem[];
   __shared__ int s_edges[kRbMaxSide];
