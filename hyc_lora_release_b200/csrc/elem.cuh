@@ -81,6 +81,62 @@ __device__ __forceinline__ void st_any(void* p, int64_t at, int type, float v) {
   else reinterpret_cast<__nv_bfloat16*>(p)[at] = __float2bfloat16_rn(v);
 }
 
+// ---- pairs of fp32 values in one 64-bit register pair: two operations per instruction
+typedef uint64_t f32x2;
+__device__ __forceinline__ f32x2 pair(float lo, float hi) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(f32x2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ f32x2 both(float v) { return pair(v, v); }
+__device__ __forceinline__ f32x2 add2f(f32x2 a, f32x2 b) { f32x2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ f32x2 mul2f(f32x2 a, f32x2 b) { f32x2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ f32x2 fma2f(f32x2 a, f32x2 b, f32x2 c) { f32x2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+
+// four adjacent values as two pairs: 8 bytes of 16-bit elements, 16 of fp32
+template <typename T> struct Quad { uint2 v; };
+template <> struct Quad<float> { uint4 v; };
+template <typename T> __device__ __forceinline__ Quad<T> ld_quad(const T* p) {
+  Quad<T> q;
+  q.v = *reinterpret_cast<const decltype(q.v)*>(p);
+  return q;
+}
+__device__ __forceinline__ void quad_to_f32(const Quad<__nv_bfloat16>& q, f32x2 (&f)[2]) {
+  f[0] = pair(bf16lo_to_f32(q.v.x), bf16hi_to_f32(q.v.x));
+  f[1] = pair(bf16lo_to_f32(q.v.y), bf16hi_to_f32(q.v.y));
+}
+__device__ __forceinline__ void quad_to_f32(const Quad<__half>& q, f32x2 (&f)[2]) {
+  const float2 a = half2_bits_to_f32(q.v.x), b = half2_bits_to_f32(q.v.y);
+  f[0] = pair(a.x, a.y);
+  f[1] = pair(b.x, b.y);
+}
+__device__ __forceinline__ void quad_to_f32(const Quad<float>& q, f32x2 (&f)[2]) {
+  f[0] = pair(__uint_as_float(q.v.x), __uint_as_float(q.v.y));
+  f[1] = pair(__uint_as_float(q.v.z), __uint_as_float(q.v.w));
+}
+__device__ __forceinline__ void st_quad(__nv_bfloat16* p, const f32x2 (&f)[2]) {
+  const float2 a = unpair(f[0]), b = unpair(f[1]);
+  *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2_rn(a.x, a.y), pack_bf16x2_rn(b.x, b.y));
+}
+__device__ __forceinline__ void st_quad(__half* p, const f32x2 (&f)[2]) {
+  const float2 a = unpair(f[0]), b = unpair(f[1]);
+  *reinterpret_cast<uint2*>(p) = make_uint2(f32_to_half2_bits(a.x, a.y), f32_to_half2_bits(b.x, b.y));
+}
+__device__ __forceinline__ void st_quad(float* p, const f32x2 (&f)[2]) {
+  const float2 a = unpair(f[0]), b = unpair(f[1]);
+  *reinterpret_cast<float4*>(p) = make_float4(a.x, a.y, b.x, b.y);
+}
+__device__ __forceinline__ void ld_any4(const void* p, int64_t at, int type, f32x2 (&f)[2]) {
+  if (type == HYC_F32) quad_to_f32(ld_quad(reinterpret_cast<const float*>(p) + at), f);
+  else if (type == HYC_F16) quad_to_f32(ld_quad(reinterpret_cast<const __half*>(p) + at), f);
+  else quad_to_f32(ld_quad(reinterpret_cast<const __nv_bfloat16*>(p) + at), f);
+}
+
 inline bool elem_type_ok(int t) { return t == HYC_BF16 || t == HYC_F16 || t == HYC_F32; }
 inline int elem_bytes(int t) { return t == HYC_F32 ? 4 : 2; }
 

@@ -7,9 +7,9 @@
 // The row sums r needs are taken again from x, which backward reads anyway: nothing is kept between the passes but q and k.
 // Everything is fp32 between the loads and the one rounding at the store.
 //
-// Bound by memory: x is read and y written once (backward: x, dy, dx).  A head belongs to G = 1 .. 32 adjacent lanes, each
-// with the 16 channels [8 i, 8 i + 8) and their partners h further (behind rot: 16 channels in a row), so that the pairs of the
-// rotation meet in one lane, all accesses are 128 bits wide, and a mean is log2 G shuffles.  A warp keeps to one of the two
+// Bound by memory: x is read and y written once (backward: x, dy, dx).  A head belongs to G = 2 .. 32 adjacent lanes, each
+// with the channels [4 i, 4 i + 4) and their partners h further (behind rot: 8 channels in a row), so that the pairs of the
+// rotation meet in one lane and a mean is log2 G shuffles; the arithmetic is on pairs of fp32 values, two per instruction.  A warp keeps to one of the two
 // tensors, so that the norm's weight, and in backward its gradient, stay in registers; the angles are loaded once per token
 // and used for the heads that the warp takes of it.  Backward's gradients of the weights: per lane over all its heads, then
 // per block in a fixed order, then one small launch over the blocks: the same bits on every run.
@@ -19,6 +19,14 @@
 namespace hyc {
 
 constexpr int kQkThreads = 256, kQkWarps = kQkThreads / 32;
+constexpr int kQkBwdBlocks = 3;      // blocks per SM that backward's registers are cut for and its workspace counts on
+
+// one instruction, two units in the last place (the root and the quotient, each rounded, take two dozen per head)
+__device__ __forceinline__ float qk_rsqrt(float v) {
+  float r;
+  asm("rsqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
 
 struct QkTensor {
   const void *x, *dy, *w;
@@ -38,38 +46,48 @@ struct QkParams {
   float* part;                     // backward: [blocks][d] sums of the weights' gradients, q's blocks first; or null
 };
 
-// The lane's two octets of a head: channels o1 .. o1 + 7 and o2 .. o2 + 7
-struct QkLane { int o1, o2; bool live, turned; };
-__device__ __forceinline__ QkLane qk_lane(int li, int d, int half) {
-  QkLane l;
-  l.live = li < d / 16;
-  l.turned = li < half / 8;
-  const int i = li - half / 8;
-  l.o1 = l.turned ? 8 * li : 2 * half + 16 * i;
-  l.o2 = l.turned ? l.o1 + half : l.o1 + 8;
-  if (!l.live) { l.o1 = 0; l.o2 = 0; }
+// The lane's channels of a head: NQ pairs of quads, o1 .. o1 + 3 and o2 .. o2 + 3
+template <int NQ> struct QkLane { int o1[NQ], o2[NQ]; bool live[NQ], turned[NQ]; };
+template <int NQ, int G>
+__device__ __forceinline__ QkLane<NQ> qk_lane(int li, int d, int half) {
+  QkLane<NQ> l;
+#pragma unroll
+  for (int j = 0; j < NQ; ++j) {
+    const int at = li + j * G, i = at - half / 4;
+    l.live[j] = at < d / 8;
+    l.turned[j] = at < half / 4;
+    l.o1[j] = l.turned[j] ? 4 * at : 2 * half + 8 * i;
+    l.o2[j] = l.turned[j] ? 4 * at + half : 2 * half + 8 * i + 4;
+    if (!l.live[j]) { l.o1[j] = 0; l.o2[j] = 0; }
+  }
   return l;
 }
 
-// cos and sin of a token at the lane's channels; a position outside of the tables gives NaN, and reads nothing
-__device__ __forceinline__ void qk_angles(const QkParams& p, int b, int m, const QkLane& l, float (&c)[8], float (&s)[8]) {
-  if (!l.turned) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) { c[e] = 1.f; s[e] = 0.f; }
-    return;
-  }
+// cos, sin and -sin of a token at the lane's channels; a position outside of the tables gives NaN, and reads nothing
+template <int NQ> struct QkAngles { f32x2 c[NQ][2], s[NQ][2], ns[NQ][2]; };
+template <int NQ>
+__device__ __forceinline__ void qk_angles(const QkParams& p, int b, int m, const QkLane<NQ>& l, QkAngles<NQ>& a) {
   int64_t at = m;
   if (p.pos != nullptr) {
     const int64_t i = b * p.pb + m * p.pm;
     at = p.pos64 ? reinterpret_cast<const int64_t*>(p.pos)[i] : (int64_t)reinterpret_cast<const int32_t*>(p.pos)[i];
   }
-  if (at < 0 || at >= p.table_rows) {
+  const bool known = at >= 0 && at < p.table_rows;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) { c[e] = __int_as_float(0x7fc00000); s[e] = c[e]; }
-    return;
+  for (int j = 0; j < NQ; ++j) {
+    a.c[j][0] = a.c[j][1] = both(1.f);
+    a.s[j][0] = a.s[j][1] = both(0.f);
+    if (l.turned[j]) {
+      if (known) {
+        ld_any4(p.cos_t, at * p.ld_cos + l.o1[j], p.table_type, a.c[j]);
+        ld_any4(p.sin_t, at * p.ld_sin + l.o1[j], p.table_type, a.s[j]);
+      } else {
+        a.c[j][0] = a.c[j][1] = a.s[j][0] = a.s[j][1] = both(__int_as_float(0x7fc00000));
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) a.ns[j][e] = a.s[j][e] ^ 0x8000000080000000ull;
   }
-  ld_any8(p.cos_t, at * p.ld_cos + l.o1, p.table_type, c);
-  ld_any8(p.sin_t, at * p.ld_sin + l.o1, p.table_type, s);
 }
 
 template <int G>
@@ -78,9 +96,23 @@ __device__ __forceinline__ float qk_sum(float v) {
   for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
+__device__ __forceinline__ float qk_total(f32x2 v) {
+  const float2 t = unpair(v);
+  return t.x + t.y;
+}
+// where a warp's items lie
+struct QkItem { uint32_t token; int first, b, m; };
+__device__ __forceinline__ QkItem qk_item(const QkParams& p, const QkTensor& t, uint32_t item) {
+  QkItem i;
+  i.token = item / (uint32_t)t.splits;
+  i.first = (int)(item - i.token * (uint32_t)t.splits) * t.per_split;
+  i.b = (int)(i.token / (uint32_t)p.seq);
+  i.m = (int)(i.token - (uint32_t)i.b * (uint32_t)p.seq);
+  return i;
+}
 
-// UNROLL head groups are on their way at once
-template <typename T, int G, int UNROLL>
+// UNROLL head groups are on their way at any time
+template <typename T, int G, int NQ, int UNROLL>
 __global__ void __launch_bounds__(kQkThreads)
 qk_norm_fwd_kernel(const __grid_constant__ QkParams p) {
   pdl_wait();
@@ -89,125 +121,176 @@ qk_norm_fwd_kernel(const __grid_constant__ QkParams p) {
   const QkTensor& t = p.t[second ? 1 : 0];
   const int block = (int)blockIdx.x - (second ? p.t[0].blocks : 0);
   const int lane = threadIdx.x & 31, sub = lane / G;
-  const QkLane l = qk_lane(lane % G, p.d, p.half);
-  const T* x = reinterpret_cast<const T*>(t.x);
-  T* out = reinterpret_cast<T*>(t.out);
-  float w1[8], w2[8];
-  ld_any8(t.w, l.o1, p.w_type, w1);
-  ld_any8(t.w, l.o2, p.w_type, w2);
+  const QkLane<NQ> l = qk_lane<NQ, G>(lane % G, p.d, p.half);
+  f32x2 w1[NQ][2], w2[NQ][2];
+#pragma unroll
+  for (int j = 0; j < NQ; ++j) {
+    ld_any4(t.w, l.o1[j], p.w_type, w1[j]);
+    ld_any4(t.w, l.o2[j], p.w_type, w2[j]);
+  }
   const float inv_d = 1.f / (float)p.d;
   const uint32_t items = (uint32_t)p.tokens * (uint32_t)t.splits;
   for (uint32_t item = (uint32_t)block * kQkWarps + (threadIdx.x >> 5); item < items; item += (uint32_t)t.blocks * kQkWarps) {
-    const uint32_t token = item / (uint32_t)t.splits;
-    const int first = (int)(item - token * (uint32_t)t.splits) * t.per_split;
-    const int b = (int)(token / (uint32_t)p.seq), m = (int)(token - (uint32_t)b * (uint32_t)p.seq);
-    const T* xt = x + b * t.xb + m * t.xm;
-    T* ot = out + (int64_t)token * t.heads * p.d;
-    float c[8], s[8];
-    qk_angles(p, b, m, l, c, s);
-    for (int g0 = first; g0 < first + t.per_split; g0 += UNROLL) {
-      Octet<T> a[UNROLL], bb[UNROLL];
+    const QkItem it = qk_item(p, t, item);
+    const T* xt = reinterpret_cast<const T*>(t.x) + it.b * t.xb + it.m * t.xm;
+    T* ot = reinterpret_cast<T*>(t.out) + (int64_t)it.token * t.heads * p.d;
+    QkAngles<NQ> a;
+    qk_angles<NQ>(p, it.b, it.m, l, a);
+    const int head0 = it.first * PER + sub;
+    int left = min((it.first + t.per_split) * PER, t.heads) - head0;      // heads of this lane's kind: left > u PER
+    const T* src = xt + head0 * t.xh;
+    T* dst = ot + head0 * p.d;
+    const int64_t step = PER * t.xh;
+    const int out_step = PER * p.d;
+    Quad<T> x1[UNROLL][NQ], x2[UNROLL][NQ];
+    auto fetch = [&](int u, bool there) {
+#pragma unroll
+      for (int j = 0; j < NQ; ++j)
+        if (l.live[j] && there) {
+          x1[u][j] = ld_quad(src + l.o1[j]);
+          x2[u][j] = ld_quad(src + l.o2[j]);
+        }
+      src += step;
+    };
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) fetch(u, left > u * PER);
+    for (; left > -sub; left -= UNROLL * PER) {
 #pragma unroll
       for (int u = 0; u < UNROLL; ++u) {
-        const int head = (g0 + u) * PER + sub;
-        const bool ok = l.live && head < t.heads && g0 + u < first + t.per_split;
-        a[u] = ok ? ld_octet(xt + head * t.xh + l.o1) : zero_octet<T>();
-        bb[u] = ok ? ld_octet(xt + head * t.xh + l.o2) : zero_octet<T>();
-      }
+        f32x2 f1[NQ][2], f2[NQ][2], ss = both(0.f);
 #pragma unroll
-      for (int u = 0; u < UNROLL; ++u) {
-        const int head = (g0 + u) * PER + sub;
-        const bool ok = l.live && head < t.heads && g0 + u < first + t.per_split;
-        float f1[8], f2[8], ss = 0.f;
-        octet_to_f32(a[u], f1);
-        octet_to_f32(bb[u], f2);
+        for (int j = 0; j < NQ; ++j) {
+          quad_to_f32(x1[u][j], f1[j]);
+          quad_to_f32(x2[u][j], f2[j]);
+          f32x2 s = both(0.f);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(f1[e], f1[e], fmaf(f2[e], f2[e], ss));
-        const float r = 1.f / sqrtf(fmaf(qk_sum<G>(ss), inv_d, p.eps));
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float n1 = f1[e] * r * w1[e], n2 = f2[e] * r * w2[e];
-          f1[e] = n1 * c[e] - n2 * s[e];
-          f2[e] = n2 * c[e] + n1 * s[e];
+          for (int e = 0; e < 2; ++e) s = fma2f(f1[j][e], f1[j][e], fma2f(f2[j][e], f2[j][e], s));
+          if (l.live[j]) ss = add2f(ss, s);
         }
-        if (ok) {
-          st_octet(ot + head * p.d + l.o1, f1);
-          st_octet(ot + head * p.d + l.o2, f2);
+        fetch(u, left > (UNROLL + u) * PER);      // its place is free: the heads UNROLL groups on
+        const float r = qk_rsqrt(fmaf(qk_sum<G>(qk_total(ss)), inv_d, p.eps));
+        const f32x2 rr = both(r);
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) {
+          f32x2 y1[2], y2[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const f32x2 n1 = mul2f(mul2f(f1[j][e], rr), w1[j][e]), n2 = mul2f(mul2f(f2[j][e], rr), w2[j][e]);
+            y1[e] = fma2f(n2, a.ns[j][e], mul2f(n1, a.c[j][e]));
+            y2[e] = fma2f(n1, a.s[j][e], mul2f(n2, a.c[j][e]));
+          }
+          if (l.live[j] && left > u * PER) {
+            st_quad(dst + l.o1[j], y1);
+            st_quad(dst + l.o2[j], y2);
+          }
         }
+        dst += out_step;
       }
     }
   }
 }
 
-template <typename T, int G>
-__global__ void __launch_bounds__(kQkThreads)
+template <typename T, int G, int NQ>
+__global__ void __launch_bounds__(kQkThreads, NQ == 1 ? kQkBwdBlocks : 1)
 qk_norm_bwd_kernel(const __grid_constant__ QkParams p) {
-  __shared__ float s_part[kQkWarps][512];
+  __shared__ float s_part[kQkWarps][8 * G * NQ];
   pdl_wait();
   constexpr int PER = 32 / G;
   const bool second = (int)blockIdx.x >= p.t[0].blocks;
   const QkTensor& t = p.t[second ? 1 : 0];
   const int block = (int)blockIdx.x - (second ? p.t[0].blocks : 0);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane / G;
-  const QkLane l = qk_lane(lane % G, p.d, p.half);
-  const T *x = reinterpret_cast<const T*>(t.x), *dy = reinterpret_cast<const T*>(t.dy);
-  T* out = reinterpret_cast<T*>(t.out);
-  float w1[8], w2[8], dw1[8], dw2[8];
-  ld_any8(t.w, l.o1, p.w_type, w1);
-  ld_any8(t.w, l.o2, p.w_type, w2);
+  const QkLane<NQ> l = qk_lane<NQ, G>(lane % G, p.d, p.half);
+  f32x2 w1[NQ][2], w2[NQ][2], dw1[NQ][2], dw2[NQ][2];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) { dw1[e] = 0.f; dw2[e] = 0.f; }
+  for (int j = 0; j < NQ; ++j) {
+    ld_any4(t.w, l.o1[j], p.w_type, w1[j]);
+    ld_any4(t.w, l.o2[j], p.w_type, w2[j]);
+    dw1[j][0] = dw1[j][1] = dw2[j][0] = dw2[j][1] = both(0.f);
+  }
   const float inv_d = 1.f / (float)p.d;
   const uint32_t items = (uint32_t)p.tokens * (uint32_t)t.splits;
   for (uint32_t item = (uint32_t)block * kQkWarps + warp; item < items; item += (uint32_t)t.blocks * kQkWarps) {
-    const uint32_t token = item / (uint32_t)t.splits;
-    const int first = (int)(item - token * (uint32_t)t.splits) * t.per_split;
-    const int b = (int)(token / (uint32_t)p.seq), m = (int)(token - (uint32_t)b * (uint32_t)p.seq);
-    const T *xt = x + b * t.xb + m * t.xm, *gt = dy + b * t.gb + m * t.gm;
-    T* ot = out + (int64_t)token * t.heads * p.d;
-    float c[8], s[8];
-    qk_angles(p, b, m, l, c, s);
-    for (int g0 = first; g0 < first + t.per_split; ++g0) {
-      const int head = g0 * PER + sub;
-      const bool ok = l.live && head < t.heads;
-      float f1[8], f2[8], g1[8], g2[8], ss = 0.f, sg = 0.f;
-      {
-        const Octet<T> xa = ok ? ld_octet(xt + head * t.xh + l.o1) : zero_octet<T>(), xb = ok ? ld_octet(xt + head * t.xh + l.o2) : zero_octet<T>();
-        const Octet<T> ga = ok ? ld_octet(gt + head * t.gh + l.o1) : zero_octet<T>(), gb = ok ? ld_octet(gt + head * t.gh + l.o2) : zero_octet<T>();
-        octet_to_f32(xa, f1); octet_to_f32(xb, f2); octet_to_f32(ga, g1); octet_to_f32(gb, g2);
-      }
+    const QkItem it = qk_item(p, t, item);
+    const T *xt = reinterpret_cast<const T*>(t.x) + it.b * t.xb + it.m * t.xm, *gt = reinterpret_cast<const T*>(t.dy) + it.b * t.gb + it.m * t.gm;
+    T* ot = reinterpret_cast<T*>(t.out) + (int64_t)it.token * t.heads * p.d;
+    QkAngles<NQ> a;
+    qk_angles<NQ>(p, it.b, it.m, l, a);
+    const int head0 = it.first * PER + sub;
+    int left = min((it.first + t.per_split) * PER, t.heads) - head0;
+    const T *src = xt + head0 * t.xh, *grad = gt + head0 * t.gh;
+    T* dst = ot + head0 * p.d;
+    const int64_t step = PER * t.xh, grad_step = PER * t.gh;
+    const int out_step = PER * p.d;
+    Quad<T> x1[NQ], x2[NQ], d1[NQ], d2[NQ];
+    auto fetch = [&](bool there) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float a = g1[e] * c[e] + g2[e] * s[e], d = g2[e] * c[e] - g1[e] * s[e];
-        g1[e] = a; g2[e] = d;
-        ss = fmaf(f1[e], f1[e], fmaf(f2[e], f2[e], ss));
-        sg = fmaf(a * w1[e], f1[e], fmaf(d * w2[e], f2[e], sg));
-      }
-      const float r = 1.f / sqrtf(fmaf(qk_sum<G>(ss), inv_d, p.eps));
-      const float mean = qk_sum<G>(sg) * r * inv_d;
+      for (int j = 0; j < NQ; ++j)
+        if (l.live[j] && there) {
+          x1[j] = ld_quad(src + l.o1[j]); x2[j] = ld_quad(src + l.o2[j]);
+          d1[j] = ld_quad(grad + l.o1[j]); d2[j] = ld_quad(grad + l.o2[j]);
+        }
+      src += step;
+      grad += grad_step;
+    };
+    fetch(left > 0);
+    for (; left > -sub; left -= PER) {
+      const bool ok = left > 0;
+      f32x2 f1[NQ][2], f2[NQ][2], g1[NQ][2], g2[NQ][2], ss = both(0.f), sg = both(0.f);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float n1 = f1[e] * r, n2 = f2[e] * r;
-        if (ok) { dw1[e] = fmaf(g1[e], n1, dw1[e]); dw2[e] = fmaf(g2[e], n2, dw2[e]); }      // (an idle lane: its NaN angles times zero)
-        f1[e] = r * (g1[e] * w1[e] - n1 * mean);
-        f2[e] = r * (g2[e] * w2[e] - n2 * mean);
+      for (int j = 0; j < NQ; ++j) {
+        quad_to_f32(x1[j], f1[j]); quad_to_f32(x2[j], f2[j]); quad_to_f32(d1[j], g1[j]); quad_to_f32(d2[j], g2[j]);
       }
-      if (ok) {
-        st_octet(ot + head * p.d + l.o1, f1);
-        st_octet(ot + head * p.d + l.o2, f2);
+      fetch(left > PER);      // the next heads while these are computed
+#pragma unroll
+      for (int j = 0; j < NQ; ++j) {
+        f32x2 s1 = both(0.f), s2 = both(0.f);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const f32x2 u = fma2f(g2[j][e], a.s[j][e], mul2f(g1[j][e], a.c[j][e])), v = fma2f(g1[j][e], a.ns[j][e], mul2f(g2[j][e], a.c[j][e]));
+          g1[j][e] = u; g2[j][e] = v;
+          s1 = fma2f(f1[j][e], f1[j][e], fma2f(f2[j][e], f2[j][e], s1));
+          s2 = fma2f(mul2f(u, w1[j][e]), f1[j][e], fma2f(mul2f(v, w2[j][e]), f2[j][e], s2));
+        }
+        if (l.live[j]) { ss = add2f(ss, s1); sg = add2f(sg, s2); }
       }
+      const float r = qk_rsqrt(fmaf(qk_sum<G>(qk_total(ss)), inv_d, p.eps));
+      const float mean = qk_sum<G>(qk_total(sg)) * r * inv_d;
+      const f32x2 rr = both(r), nm = both(-mean);
+#pragma unroll
+      for (int j = 0; j < NQ; ++j) {
+        f32x2 y1[2], y2[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const f32x2 n1 = mul2f(f1[j][e], rr), n2 = mul2f(f2[j][e], rr);
+          if (ok) { dw1[j][e] = fma2f(g1[j][e], n1, dw1[j][e]); dw2[j][e] = fma2f(g2[j][e], n2, dw2[j][e]); }
+          y1[e] = mul2f(rr, fma2f(n1, nm, mul2f(g1[j][e], w1[j][e])));
+          y2[e] = mul2f(rr, fma2f(n2, nm, mul2f(g2[j][e], w2[j][e])));
+        }
+        if (ok && l.live[j]) {
+          st_quad(dst + l.o1[j], y1);
+          st_quad(dst + l.o2[j], y2);
+        }
+      }
+      dst += out_step;
     }
   }
   if (p.part == nullptr) return;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
+  for (int j = 0; j < NQ; ++j)
 #pragma unroll
-    for (int o = G; o < 32; o <<= 1) {
-      dw1[e] += __shfl_xor_sync(0xffffffffu, dw1[e], o);
-      dw2[e] += __shfl_xor_sync(0xffffffffu, dw2[e], o);
+    for (int e = 0; e < 2; ++e) {
+#pragma unroll
+      for (int o = G; o < 32; o <<= 1) {
+        dw1[j][e] = add2f(dw1[j][e], __shfl_xor_sync(0xffffffffu, (unsigned long long)dw1[j][e], o));
+        dw2[j][e] = add2f(dw2[j][e], __shfl_xor_sync(0xffffffffu, (unsigned long long)dw2[j][e], o));
+      }
+      if (sub == 0 && l.live[j]) {
+        const float2 u = unpair(dw1[j][e]), v = unpair(dw2[j][e]);
+        s_part[warp][l.o1[j] + 2 * e] = u.x; s_part[warp][l.o1[j] + 2 * e + 1] = u.y;
+        s_part[warp][l.o2[j] + 2 * e] = v.x; s_part[warp][l.o2[j] + 2 * e + 1] = v.y;
+      }
     }
-    if (sub == 0 && l.live) { s_part[warp][l.o1 + e] = dw1[e]; s_part[warp][l.o2 + e] = dw2[e]; }
-  }
   __syncthreads();
   for (int i = threadIdx.x; i < p.d; i += kQkThreads) {
     float sum = 0.f;
@@ -264,15 +347,15 @@ static int qk_check(const hyc_qk_norm* a, bool backward) {
   return HYC_OK;
 }
 
-// lanes of a head
+// lanes of a head: one per eight channels, a power of two; 32 of them with twice as many above 256 channels
 static int qk_group(int d) {
-  int g = 1;
-  while (g < d / 16) g <<= 1;
+  int g = 2;
+  while (g < d / 8 && g < 32) g <<= 1;
   return g;
 }
 
 // Blocks for the two tensors in proportion to their heads, at most one resident wave and no more than there is work for; a token's head
-// groups are dealt to several warps where there are fewer tokens than warps.
+// groups are dealt to several warps where that evens out what the warps have to do.
 static void qk_plan(QkParams& p, int wave) {
   const int per = 32 / qk_group(p.d), heads = p.t[0].heads + p.t[1].heads;
   for (int i = 0; i < 2; ++i) {
@@ -280,11 +363,14 @@ static void qk_plan(QkParams& p, int wave) {
     const int groups = (t.heads + per - 1) / per;
     int blocks = (int)((int64_t)wave * t.heads / heads);
     if (blocks < 1) blocks = 1;
+    // a warp's share is a whole number of items: small ones fill the last round, each costs about two groups more (division, angles)
     const int64_t warps = (int64_t)blocks * kQkWarps;
-    int64_t splits = p.tokens >= warps ? 1 : (warps + p.tokens - 1) / p.tokens;
-    if (splits > groups) splits = groups;
-    t.per_split = (int)((groups + splits - 1) / splits);
-    t.splits = (groups + t.per_split - 1) / t.per_split;
+    int64_t best = 0;
+    for (int per_split = 1; per_split <= groups; ++per_split) {
+      const int splits = (groups + per_split - 1) / per_split;
+      const int64_t cost = ((int64_t)p.tokens * splits + warps - 1) / warps * (per_split + 2);
+      if (best == 0 || cost <= best) { best = cost; t.per_split = per_split; t.splits = splits; }
+    }
     const int64_t need = ((int64_t)p.tokens * t.splits + kQkWarps - 1) / kQkWarps;
     t.blocks = (int)(need < blocks ? need : blocks);
   }
@@ -306,25 +392,24 @@ static void qk_fill(QkParams& p, const hyc_qk_norm* a) {
   p.part = nullptr;
 }
 
+// f(element, lanes of a head, pairs of quads per lane)
 template <typename F>
-static int qk_by_type(int type, int group, F&& f) {
+static int qk_by_type(int type, int d, F&& f) {
   auto by_group = [&](auto elem) -> int {
-    using T = decltype(elem);
-    switch (group) {
-      case 1: return f(elem, std::integral_constant<int, 1>());
-      case 2: return f(elem, std::integral_constant<int, 2>());
-      case 4: return f(elem, std::integral_constant<int, 4>());
-      case 8: return f(elem, std::integral_constant<int, 8>());
-      case 16: return f(elem, std::integral_constant<int, 16>());
-      default: return f(elem, std::integral_constant<int, 32>());
+    using std::integral_constant;
+    constexpr integral_constant<int, 1> one{};
+    switch (qk_group(d)) {
+      case 2: return f(elem, integral_constant<int, 2>(), one);
+      case 4: return f(elem, integral_constant<int, 4>(), one);
+      case 8: return f(elem, integral_constant<int, 8>(), one);
+      case 16: return f(elem, integral_constant<int, 16>(), one);
+      default: return d <= 256 ? f(elem, integral_constant<int, 32>(), one) : f(elem, integral_constant<int, 32>(), integral_constant<int, 2>());
     }
   };
   if (type == HYC_F32) return by_group(float());
   if (type == HYC_F16) return by_group(__half());
   return by_group(__nv_bfloat16());
 }
-
-constexpr int kQkBwdWave = 4;      // resident blocks per SM that backward counts on at most (its workspace does not ask the device)
 
 }  // namespace hyc
 
@@ -335,8 +420,8 @@ extern "C" HYC_API int hyc_qk_norm_rope_fwd(const hyc_qk_norm* a, void* stream) 
   if (rc != HYC_OK || a->batch * a->seq == 0) return rc;
   QkParams p;
   qk_fill(p, a);
-  return qk_by_type(a->type, qk_group(p.d), [&](auto elem, auto group) -> int {
-    auto kern = qk_norm_fwd_kernel<decltype(elem), decltype(group)::value, sizeof(elem) == 4 ? 1 : 2>;
+  return qk_by_type(a->type, p.d, [&](auto elem, auto group, auto quads) -> int {
+    auto kern = qk_norm_fwd_kernel<decltype(elem), decltype(group)::value, decltype(quads)::value, 2>;
     qk_plan(p, num_sms() * resident_blocks(kern, kQkThreads, 0, 2));
     launch_pdl(kern, dim3((unsigned)(p.t[0].blocks + p.t[1].blocks)), dim3(kQkThreads), 0, (cudaStream_t)stream, p);
     HYC_CHECK_LAUNCH();
@@ -345,7 +430,7 @@ extern "C" HYC_API int hyc_qk_norm_rope_fwd(const hyc_qk_norm* a, void* stream) 
 }
 
 extern "C" HYC_API size_t hyc_qk_norm_rope_workspace_bytes(int head_dim) {
-  return head_dim < 16 || head_dim > 512 ? 0 : (size_t)(num_sms() * kQkBwdWave + 2) * (size_t)head_dim * sizeof(float);
+  return head_dim < 16 || head_dim > 512 ? 0 : (size_t)(num_sms() * kQkBwdBlocks + 2) * (size_t)head_dim * sizeof(float);
 }
 
 extern "C" HYC_API int hyc_qk_norm_rope_bwd(const hyc_qk_norm* a, void* dweight_q, void* dweight_k, void* workspace, size_t workspace_bytes, void* stream) {
@@ -359,10 +444,10 @@ extern "C" HYC_API int hyc_qk_norm_rope_bwd(const hyc_qk_norm* a, void* dweight_
   qk_fill(p, a);
   if (p.tokens > 0) {
     p.part = weights ? (float*)workspace : nullptr;
-    const int r = qk_by_type(a->type, qk_group(p.d), [&](auto elem, auto group) -> int {
-      auto kern = qk_norm_bwd_kernel<decltype(elem), decltype(group)::value>;
-      const int res = resident_blocks(kern, kQkThreads, 0, 2);
-      qk_plan(p, num_sms() * (res < kQkBwdWave ? res : kQkBwdWave));
+    const int r = qk_by_type(a->type, p.d, [&](auto elem, auto group, auto quads) -> int {
+      auto kern = qk_norm_bwd_kernel<decltype(elem), decltype(group)::value, decltype(quads)::value>;
+      const int res = resident_blocks(kern, kQkThreads, 0, 1);
+      qk_plan(p, num_sms() * (res < kQkBwdBlocks ? res : kQkBwdBlocks));
       launch_pdl(kern, dim3((unsigned)(p.t[0].blocks + p.t[1].blocks)), dim3(kQkThreads), 0, (cudaStream_t)stream, p);
       HYC_CHECK_LAUNCH();
       return HYC_OK;
