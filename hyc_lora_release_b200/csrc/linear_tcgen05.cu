@@ -12,9 +12,9 @@
 // rows and any multiple of 8 columns is right), every wait bounded (hyc_linear_status):
 //   tiles    persistent CTA pairs, 256 x 256 or 256 x 128 results per pair by tcgen05.mma.cta_group::2, two accumulators, so that the
 //            epilogue of one tile overlaps the main loop of the next
-//   slices   few rows or few tiles: one tile of 256 result COLUMNS x up to 256 rows per CTA pair, the columns on the 256 lanes of tensor
-//            memory and the rows in its columns (a product of one row costs N = 16, not 128), K shared by the pairs of a cluster, whose
-//            partial sums meet in distributed shared memory in a fixed order
+//   slices   few rows or few tiles: one tile of 128 result COLUMNS x up to 256 rows per CTA (256 per CTA pair), the columns on the lanes of
+//            tensor memory and the rows in its columns (a product of one row costs N = 16, not 128), K shared by the CTAs or pairs of a
+//            cluster, whose partial sums meet in distributed shared memory in a fixed order
 #include "tc_common.cuh"
 #include "elem.cuh"
 #include <type_traits>
@@ -38,11 +38,24 @@ struct Shape { int R, C, K; };
 
 // ---- activations, fp32
 __device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
+// erfc(|x| / sqrt 2) / 2 = q(t) e^(-x^2 / 2), t = 1 / (1 + p |x| / sqrt 2): the rational approximation 7.1.26 of Abramowitz and Stegun's
+// Handbook, off by 7.5e-8 at most (half of erf's 1.5e-7).  x Phi(x) = max(x, 0) - |x| erfc(..) / 2, with no cancellation on either side.
+__device__ __forceinline__ float normal_tail(float x, float& density) {      // density: e^(-x^2 / 2)
+  const float ax = fabsf(x);
+  const float t = __fdividef(1.f, fmaf(0.3275911f * 0.70710678118654752f, ax, 1.f));
+  const float q = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f), 0.5f * 1.421413741f), 0.5f * -0.284496736f), 0.5f * 0.254829592f);
+  density = __expf(-0.5f * x * x);
+  return q * density;
+}
 constexpr float kTanhA = 1.5957691216057308f, kTanhB = 0.0713548162726009f;      // 2 sqrt(2 / pi), the same times 0.044715
 template <int ACT>
 __device__ __forceinline__ float act_of(float x) {
   if constexpr (ACT == HYC_ACT_RELU) return x > 0.f || x != x ? x : 0.f;      // (NaN stays)
-  else if constexpr (ACT == HYC_ACT_GELU) return 0.5f * x * (1.f + erff(x * 0.70710678118654752f));
+  else if constexpr (ACT == HYC_ACT_GELU) {
+    float density;
+    const float tail = normal_tail(x, density);
+    return fmaf(-fminf(fabsf(x), 100.f), tail, fmaxf(x, 0.f));      // (far out the tail is 0; NaN is in it)
+  }
   else if constexpr (ACT == HYC_ACT_GELU_TANH) return x * sigmoid(x * fmaf(kTanhB, x * x, kTanhA));      // (1 + tanh u) / 2 = sigmoid(2 u)
   else if constexpr (ACT == HYC_ACT_SILU) return x * sigmoid(x);
   else return x;
@@ -50,7 +63,11 @@ __device__ __forceinline__ float act_of(float x) {
 template <int ACT>
 __device__ __forceinline__ float slope_of(float x) {
   if constexpr (ACT == HYC_ACT_RELU) return x > 0.f ? 1.f : x != x ? x : 0.f;
-  else if constexpr (ACT == HYC_ACT_GELU) return fmaf(0.5f, erff(x * 0.70710678118654752f), 0.5f) + x * 0.39894228040143268f * __expf(-0.5f * x * x);
+  else if constexpr (ACT == HYC_ACT_GELU) {
+    float density;
+    const float tail = normal_tail(x, density);
+    return fmaf(x * 0.39894228040143268f, density, x > 0.f ? 1.f - tail : tail);
+  }
   else if constexpr (ACT == HYC_ACT_GELU_TANH) {
     if (fabsf(x) > 30.f) return x > 0.f ? 1.f : 0.f;      // (x^2 may be infinite)
     const float s = sigmoid(x * fmaf(kTanhB, x * x, kTanhA));
@@ -328,14 +345,14 @@ linear_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
 }
 
 // ------------------------------------------------------------------ slices
-constexpr int S_THREADS = 64 + 128, S_STAGES_MAX = 12;
+constexpr int S_EPI_WARPS = 8, S_THREADS = 64 + 32 * S_EPI_WARPS, S_STAGES_MAX = 12;
 constexpr int S_PIPE_ONE = 196608, S_PIPE_TWO = 98304;                    // one CTA per SM, or two
 constexpr int s_smem(int pipe) { return 1024 + pipe + 512; }
 
 struct SliceParams {
   Shape s;
   Epilogue e;
-  int tn, tiles_c, split;      // result rows of a tile (a multiple of 16 up to 256), tiles of 256 columns, pairs that share K
+  int tn, tiles_c, split;      // result rows of a tile (a multiple of 16 up to 256), column tiles, CTAs (or pairs) that share K
   int stages, stage_bytes, tmem_cols;
 };
 
@@ -348,18 +365,22 @@ __device__ __forceinline__ void tc_ld16(uint32_t taddr, uint32_t (&v)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
-// 16 rows of results of the lane's column
+// the residual of 16 rows of the lane's column
 template <typename T>
-__device__ __forceinline__ void slice_block(const SliceParams& p, float (&v)[16], float bias, int row0, int rows, int64_t col) {
-  T *pre = (T*)p.e.pre, *out = (T*)p.e.out;
+__device__ __forceinline__ void slice_residual(const SliceParams& p, int row0, int rows, int64_t col, float (&r)[16]) {
   const T* res = (const T*)p.e.residual;
-  float r[16];
 #pragma unroll
   for (int j = 0; j < 16; ++j) {
     r[j] = 0.f;
-    if (res != nullptr && j < rows) r[j] = to_f32(res[(int64_t)(row0 + j) * p.e.ld_res + col]);
-    v[j] += bias;
+    if (res != nullptr && j < rows && col < p.s.C) r[j] = to_f32(res[(int64_t)(row0 + j) * p.e.ld_res + col]);
   }
+}
+// 16 rows of results of the lane's column
+template <typename T>
+__device__ __forceinline__ void slice_block(const SliceParams& p, float (&v)[16], const float (&r)[16], float bias, int row0, int rows, int64_t col) {
+  T *pre = (T*)p.e.pre, *out = (T*)p.e.out;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) v[j] += bias;
   if (pre != nullptr) {
 #pragma unroll
     for (int j = 0; j < 16; ++j)
@@ -374,23 +395,30 @@ __device__ __forceinline__ void slice_block(const SliceParams& p, float (&v)[16]
     if (j < rows) out[(int64_t)(row0 + j) * p.s.C + col] = from_f32<T>(v[j] + r[j]);
 }
 
-// C_MN: the operand that gives the result's columns (B of the product) is MN-major; R_MN: the one that gives its rows (A)
-template <typename T, bool C_MN, bool R_MN>
+// C_MN: the operand that gives the result's columns (B of the product) is MN-major; R_MN: the one that gives its rows (A).  PAIR: two CTAs
+// share a tile of 256 columns, each loading half of the rows' operand; else a CTA has a tile of 128 columns of its own.
+template <typename T, bool C_MN, bool R_MN, bool PAIR>
 __global__ void __launch_bounds__(S_THREADS)
 linear_slices_kernel(const __grid_constant__ CUtensorMap map_c, const __grid_constant__ CUtensorMap map_r, const SliceParams p) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full[S_STAGES_MAX], empty[S_STAGES_MAX], acc_full;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
+  constexpr int CTAS = PAIR ? 2 : 1;
   uint8_t* smem = align_shared(smem_raw);
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
-  const int crank = (int)cluster_ctarank(), half = crank & 1, slice = crank >> 1;
-  const uint32_t leader = (uint32_t)(crank & ~1);
-  const int tile = (int)blockIdx.x / (2 * p.split), tc = tile % p.tiles_c, tr = tile / p.tiles_c;
-  const int c0 = tc * 2 * BM + half * BM, r0 = tr * p.tn, rh = p.tn / 2;
+  const bool clustered = CTAS * p.split > 1;
+  const int crank = clustered ? (int)cluster_ctarank() : 0, half = PAIR ? crank & 1 : 0, slice = PAIR ? crank >> 1 : crank;
+  const uint32_t leader = (uint32_t)(PAIR ? crank & ~1 : crank);
+  const int tile = (int)blockIdx.x / (CTAS * p.split), tc = tile % p.tiles_c, tr = tile / p.tiles_c;
+  const int c0 = (tc * CTAS + half) * BM, r0 = tr * p.tn, rh = p.tn / CTAS;
   const int kbs = (p.s.K + BK - 1) / BK;
   const int kb_lo = (int)((int64_t)kbs * slice / p.split), kb_hi = (int)((int64_t)kbs * (slice + 1) / p.split);
 
+  if (warp == 0 && elect_one()) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_c)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_r)) : "memory");
+  }
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
     mbar_init(&acc_full, 1);
@@ -399,12 +427,17 @@ linear_slices_kernel(const __grid_constant__ CUtensorMap map_c, const __grid_con
   }
   pdl_wait();      // before tensor memory is taken: see launch_pdl
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(p.tmem_cols) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    if (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(p.tmem_cols) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(p.tmem_cols) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
   }
   tc_fence_before();
   __syncthreads();
-  cluster_sync_all();      // the peer's barriers exist before anything is signalled there
+  if (PAIR) cluster_sync_all();      // the peer's barriers exist before anything is signalled there
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
   volatile int* flag = &abort_flag;
@@ -412,10 +445,12 @@ linear_slices_kernel(const __grid_constant__ CUtensorMap map_c, const __grid_con
     if (lane == 0 && !*flag) { *flag = 1; atomicExch(&g_status, code); }
   };
   float* part = reinterpret_cast<float*>(smem);      // [row][column] partial sums, over the drained stages
-  const int quad = warp & 3;
+  const int quad = warp & 3, row_half = (warp - 2) >> 2;      // epilogue: 32 columns, and every other block of 16 rows
   const int64_t col = (int64_t)c0 + quad * 32 + lane;
   const uint32_t t_lane = tmem + ((uint32_t)(quad * 32) << 16);
-  float bias = 0.f;
+  // the epilogue's blocks of 16 rows, dealt to the slices and their two groups of warps in turn
+  const int end = min(p.s.R - r0, p.tn), first_row = 16 * (2 * slice + row_half), row_step = 32 * p.split;
+  float bias = 0.f, res[16];
   bool ok = true;
 
   if (warp == 0) {
@@ -423,20 +458,20 @@ linear_slices_kernel(const __grid_constant__ CUtensorMap map_c, const __grid_con
     uint32_t phase = 0;
     for (int kb = kb_lo; kb < kb_hi; ++kb) {
       if (!mbar_wait_warp(&empty[stage], phase ^ 1u, flag)) { give_up(ST_TIMEOUT_PRODUCER); break; }
-      const uint32_t sc = smem_u32(smem + stage * p.stage_bytes), sr = sc + STAGE_A_BYTES, bar = map_to_cta(&full[stage], leader);
+      const uint32_t sc = smem_u32(smem + stage * p.stage_bytes), sr = sc + STAGE_A_BYTES, bar = PAIR ? map_to_cta(&full[stage], leader) : smem_u32(&full[stage]);
       const int k0 = kb * BK, rr = r0 + half * rh;
       if (elect_one()) {
-        if (half == 0) mbar_expect_tx(&full[stage], (uint32_t)(2 * (STAGE_A_BYTES + rh * BK * 2)));
+        if (half == 0) mbar_expect_tx(&full[stage], (uint32_t)(CTAS * (STAGE_A_BYTES + rh * BK * 2)));
         if (C_MN) {
-          tma_load_2d<true>(sc, &map_c, bar, c0, k0);
-          tma_load_2d<true>(sc + 8192, &map_c, bar, c0 + 64, k0);
+          tma_load_2d<PAIR>(sc, &map_c, bar, c0, k0);
+          tma_load_2d<PAIR>(sc + 8192, &map_c, bar, c0 + 64, k0);
         } else {
-          tma_load_2d<true>(sc, &map_c, bar, k0, c0);
+          tma_load_2d<PAIR>(sc, &map_c, bar, k0, c0);
         }
         if (R_MN) {
-          for (int j = 0; j < rh; j += 64) tma_load_2d<true>(sr + (uint32_t)(j * 128), &map_r, bar, rr + j, k0);
+          for (int j = 0; j < rh; j += 64) tma_load_2d<PAIR>(sr + (uint32_t)(j * 128), &map_r, bar, rr + j, k0);
         } else {
-          tma_load_2d<true>(sr, &map_r, bar, k0, rr);
+          tma_load_2d<PAIR>(sr, &map_r, bar, k0, rr);
         }
       }
       __syncwarp();
@@ -444,7 +479,7 @@ linear_slices_kernel(const __grid_constant__ CUtensorMap map_c, const __grid_con
     }
   } else if (warp == 1) {
     if (half == 0) {
-      const uint32_t idesc = instruction<T, C_MN, R_MN>(2 * BM, p.tn);
+      const uint32_t idesc = instruction<T, C_MN, R_MN>(CTAS * BM, p.tn);
       int stage = 0;
       uint32_t phase = 0;
       bool fine = true;
@@ -455,17 +490,18 @@ linear_slices_kernel(const __grid_constant__ CUtensorMap map_c, const __grid_con
         const uint64_t a = operand_desc<C_MN>(sc), b = operand_desc<R_MN>(sc + STAGE_A_BYTES);
         if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < BK / 16; ++kk) tc_mma<true>(tmem, a + kk * kStep<C_MN>, b + kk * kStep<R_MN>, idesc, (kb > kb_lo || kk > 0) ? 1u : 0u);
-          tc_commit<true>(&empty[stage], leader);
+          for (int kk = 0; kk < BK / 16; ++kk) tc_mma<PAIR>(tmem, a + kk * kStep<C_MN>, b + kk * kStep<R_MN>, idesc, (kb > kb_lo || kk > 0) ? 1u : 0u);
+          tc_commit<PAIR>(&empty[stage], leader);
         }
         __syncwarp();
         if (++stage == p.stages) { stage = 0; phase ^= 1u; }
       }
-      if (fine && elect_one()) tc_commit<true>(&acc_full, leader);
+      if (fine && elect_one()) tc_commit<PAIR>(&acc_full, leader);
       __syncwarp();
     }
   } else {
     if (p.e.bias != nullptr && col < p.s.C) bias = to_f32(reinterpret_cast<const T*>(p.e.bias)[col]);
+    slice_residual<T>(p, r0 + first_row, end - first_row, col, res);      // (on its way during the main loop)
     ok = mbar_wait(&acc_full, 0, flag);
     if (!ok && !*flag) { *flag = 1; atomicExch(&g_status, ST_TIMEOUT_EPILOGUE); }
     ok = __all_sync(0xffffffffu, ok);
@@ -473,7 +509,7 @@ linear_slices_kernel(const __grid_constant__ CUtensorMap map_c, const __grid_con
     if (ok && p.split > 1) {
       // the stages are drained (the accumulators are complete): they hold the partial sums now
 #pragma unroll 1
-      for (int j0 = 0; j0 < p.tn; j0 += 16) {
+      for (int j0 = 16 * row_half; j0 < p.tn; j0 += 32) {
         uint32_t v[16];
         tc_ld16(t_lane + (uint32_t)j0, v);
 #pragma unroll
@@ -484,9 +520,11 @@ linear_slices_kernel(const __grid_constant__ CUtensorMap map_c, const __grid_con
   // every CTA of the cluster has its partial sums in place (or has given up: the status says so)
   if (p.split > 1) cluster_sync_all();
   if (warp >= 2 && ok) {
-    const int end = min(p.s.R - r0, p.tn);
-    // blocks of 16 rows, dealt to the slices in turn
-    for (int j0 = 16 * slice; j0 < end; j0 += 16 * p.split) {
+    for (int j0 = first_row; j0 < end; j0 += row_step) {
+      float now[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) now[j] = res[j];
+      if (j0 + row_step < end) slice_residual<T>(p, r0 + j0 + row_step, end - j0 - row_step, col, res);
       float v[16];
       if (p.split == 1) {
         uint32_t u[16];
@@ -497,24 +535,24 @@ linear_slices_kernel(const __grid_constant__ CUtensorMap map_c, const __grid_con
 #pragma unroll
         for (int j = 0; j < 16; ++j) v[j] = 0.f;
         for (int s = 0; s < p.split; ++s) {      // rank 0, 1, ...: the same order on every run
-          const uint32_t base = map_to_cta(part + j0 * BM + quad * 32 + lane, (uint32_t)(2 * s + half));
+          const uint32_t base = map_to_cta(part + j0 * BM + quad * 32 + lane, (uint32_t)(CTAS * s + half));
+          float f[16];
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            float f;
-            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(base + (uint32_t)(j * BM * 4)));
-            v[j] += f;
-          }
+          for (int j = 0; j < 16; ++j) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f[j]) : "r"(base + (uint32_t)(j * BM * 4)));
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[j] += f[j];
         }
       }
-      if (col < p.s.C) slice_block<T>(p, v, bias, r0 + j0, end - j0, col);
+      if (col < p.s.C) slice_block<T>(p, v, now, bias, r0 + j0, end - j0, col);
     }
   }
   tc_fence_before();
   __syncthreads();
-  cluster_sync_all();      // nobody leaves while a peer may still read its partial sums or use its barriers
+  if (clustered) cluster_sync_all();      // nobody leaves while a peer may still read its partial sums or use its barriers
   if (warp == 1) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.tmem_cols) : "memory");
+    if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.tmem_cols) : "memory");
+    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.tmem_cols) : "memory");
   }
 }
 
@@ -589,7 +627,7 @@ static bool operand_map(CUtensorMap* m, const void* ptr, int type, bool mn, int6
   cuuint32_t box[2] = {64u, mn ? 64u : (cuuint32_t)box_rows};
   cuuint32_t estr[2] = {1u, 1u};
   return enc(m, type == HYC_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, estr,
-             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -619,7 +657,7 @@ static int launch_cluster(K kern, unsigned blocks, unsigned threads, unsigned cl
   at[1].id = cudaLaunchAttributeClusterDimension;
   at[1].val.clusterDim.x = cluster; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 2;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   if (cudaLaunchKernelEx(&cfg, kern, args...) != cudaSuccess) {
     hyc_set_last_cuda_error((int)cudaGetLastError());
     return HYC_ERR_LAUNCH;
@@ -627,12 +665,18 @@ static int launch_cluster(K kern, unsigned blocks, unsigned threads, unsigned cl
   return HYC_OK;
 }
 
-// ---- which kernel, by estimated cycles.  A pair's 256 x 256 x 64 k-block takes 512 (tensor pipe), a 256 x 128 one about 0.68 of it (operands
-// from L2); a slice's k-block 2 tn (tensor pipe) or 256 + tn (operands from L2).
+// ---- which kernel, by estimated cycles.  The constants were fitted to the two kernels in all their forms at fourteen sizes (1 to 1500 rows,
+// 1024 to 11008 deep and wide, cold, us):
+//              tiles   slices: best            1 / 2 / 4 CTAs share K
+//   1 x 4096 x 11008    33.6    20.5      21.3 / 20.9 / 26.9           256 x 4096 x 4096    20.3    16.8     33.2 / 23.8 / 34.1 (pairs)
+//   8 x 11008 x 4096    41.2    21.0      34.9 / 23.3 / 21.1           333 x 11008 x 4096   42.6    30.8     47.1 / 30.8 / 60.9 (pairs)
+//   64 x 4096 x 11008   27.8    22.7      23.5 / 22.7 / 30.1           512 x 4096 x 4096    21.0    22.7     34.2 / 24.9 / 49.7 (pairs)
+//   128 x 4096 x 4096   20.3    14.2      22.4 / 17.0 / 16.3           1500 x 4096 x 512    19.3    16.0     33.2 / 23.3 / 19.0 (pairs)
+// What the rule picks is 5 % from the best form on average.  (Clusters of 8 were never the best: only 15 of them are resident.)
 struct TilePlan { int n_wide, n_tiles; float cost; };
 static TilePlan plan_tiles(const Shape& s) {
   const int tiles_m = (s.R + 2 * BM - 1) / (2 * BM), halves = (s.C + BN / 2 - 1) / (BN / 2), pairs = num_sms() / 2;
-  const float block = 512.f * (float)((s.K + BK - 1) / BK), half = 0.68f;
+  const float block = 547.f * (float)((s.K + BK - 1) / BK), half = 0.71f;
   TilePlan best = {0, halves, 1e30f};
   for (int w = halves / 2; w >= 0; --w) {
     const int64_t wide = (int64_t)tiles_m * w, narrow = (int64_t)tiles_m * (halves - 2 * w);
@@ -642,29 +686,64 @@ static TilePlan plan_tiles(const Shape& s) {
       const float c = rounds + 1 + half * (float)(behind > 0 ? (behind + pairs - 1) / pairs : 0);
       if (c > rest_cost) rest_cost = c;
     }
-    const float cost = rest_cost * block + 8000.f;
+    const float cost = rest_cost * block + 14000.f;
     if (cost < best.cost * 0.98f) best = {w, halves - w, cost};
   }
+  const float stream = 2.f * (float)s.C * (float)s.K / 1500.f;      // few tiles: the loads of their pairs alone do not fill the memory's pipe
+  if (stream > best.cost) best.cost = stream;
   return best;
 }
-struct SlicePlan { int tn, split; float cost; };
+// two CTAs per SM: the partial sums, 512 bytes per row, have to fit in half of the shared memory
+static bool slice_two(int tn, bool pair) { return tn <= (pair ? 128 : 64); }
+// clusters of 4 CTAs do not reach every SM (33 of them are resident on a B200, one CTA per SM)
+static int slice_clusters(int ctas) { return ctas <= 2 ? num_sms() / ctas : num_sms() * 33 / 148; }
+struct SlicePlan { int tn, split; bool pair; float cost; };
 static SlicePlan plan_slices(const Shape& s, bool r_mn) {
-  const int tiles_c = (s.C + 2 * BM - 1) / (2 * BM), kbs = (s.K + BK - 1) / BK, sms = num_sms(), base = (s.R + 255) / 256;
-  SlicePlan best = {0, 0, 1e30f};
-  for (int more = 1; more <= 2; ++more) {
-    const int tiles_r = base * more;
-    int tn = ((s.R + tiles_r - 1) / tiles_r + 15) / 16 * 16;
-    if (r_mn) tn = tn <= 128 ? 128 : 256;
-    for (int split = 1; split <= 4; split *= 2) {
+  const int kbs = (s.K + BK - 1) / BK, base = (s.R + 255) / 256;
+  SlicePlan best = {0, 0, false, 1e30f};
+  for (int form = 0; form < 4; ++form) {
+    const bool pair = (form & 1) != 0;
+    const int ctas = pair ? 2 : 1, tiles_c = (s.C + ctas * BM - 1) / (ctas * BM), row_tiles = base << (form >> 1);
+    int tn = ((s.R + row_tiles - 1) / row_tiles + 15) / 16 * 16;
+    if (r_mn) tn = tn <= 64 && !pair ? 64 : tn <= 128 ? 128 : 256;
+    const int64_t tiles_r = (s.R + tn - 1) / tn, clusters = tiles_c * tiles_r;
+    for (int split = 1; split * ctas <= 4; split *= 2) {
       if (split > 1 && kbs < 4 * split) break;
-      const int64_t ctas = 2ll * split * tiles_c * ((s.R + tn - 1) / tn);
-      const float block = 2.f * tn > 256.f + tn ? 2.f * tn : 256.f + tn;
-      const float cost = (float)((ctas + sms - 1) / sms) * ((float)((kbs + split - 1) / split) * block + 60.f * (float)((tn + split - 1) / split)) +
-                         (split > 1 ? 3500.f : 0.f) + 3000.f;
-      if (cost < best.cost) best = {tn, split, cost};
+      const int64_t at_once = (int64_t)slice_clusters(split * ctas) * (slice_two(tn, pair) ? 2 : 1), waves = (clusters + at_once - 1) / at_once;
+      const int64_t running = (clusters < at_once ? clusters : at_once) * split * ctas;
+      const float per_sm = running > num_sms() ? (float)running / (float)num_sms() : 1.f;
+      // a k-block: the tensor pipe, operands from L2 at 64 bytes per cycle and SM, all SMs' columns once from HBM
+      const float operands = (float)(STAGE_A_BYTES + tn / ctas * BK * 2) / 64.f, hbm = (float)STAGE_A_BYTES * (float)running / 3200.f / (float)tiles_r;
+      float block = (2.f * tn > operands ? 2.f * tn : operands) * per_sm;
+      if (hbm > block) block = hbm;
+      const float cost = 9300.f + (float)waves * ((float)((kbs + split - 1) / split) * block + 50.f * (float)tn / (float)split * per_sm + 5300.f) +
+                         (split > 1 ? 3000.f + 22.f * (float)tn : 0.f);
+      if (cost < best.cost) best = {tn, split, pair, cost};
     }
   }
   return best;
+}
+
+template <typename T, bool A_MN, bool B_MN, bool PAIR>
+static int launch_slices(const hyc_linear* a, const Shape& s, const Epilogue& e, const SlicePlan& sp, cudaStream_t st) {
+  constexpr auto kern = linear_slices_kernel<T, B_MN, A_MN, PAIR>;
+  constexpr int CTAS = PAIR ? 2 : 1;
+  const int rc = more_shared_memory<kern>(s_smem(S_PIPE_ONE));
+  if (rc != HYC_OK) return rc;
+  SliceParams p;
+  p.s = s; p.e = e; p.tn = sp.tn; p.split = sp.split;
+  p.tiles_c = (s.C + CTAS * BM - 1) / (CTAS * BM);
+  const int64_t ctas = (int64_t)CTAS * p.split * p.tiles_c * ((s.R + p.tn - 1) / p.tn);
+  if (ctas > 0x7fffffff) return HYC_ERR_SHAPE;
+  const int pipe = ctas > num_sms() && slice_two(p.tn, PAIR) ? S_PIPE_TWO : S_PIPE_ONE;
+  p.stage_bytes = STAGE_A_BYTES + p.tn / CTAS * BK * 2;
+  p.stages = pipe / p.stage_bytes < S_STAGES_MAX ? pipe / p.stage_bytes : S_STAGES_MAX;
+  p.tmem_cols = 32;
+  while (p.tmem_cols < p.tn) p.tmem_cols *= 2;
+  CUtensorMap mc, mr;
+  if (!operand_map(&mc, a->b, a->type, B_MN, s.C, s.K, a->ld_b, BM) || !operand_map(&mr, a->a, a->type, A_MN, s.R, s.K, a->ld_a, p.tn / CTAS))
+    return HYC_ERR_UNSUPPORTED;
+  return launch_cluster(kern, (unsigned)ctas, S_THREADS, (unsigned)(CTAS * p.split), s_smem(pipe), st, mc, mr, p);
 }
 
 template <typename T, bool A_MN, bool B_MN>
@@ -673,24 +752,7 @@ static int launch_product(const hyc_linear* a, cudaStream_t st) {
   const Epilogue e = {a->bias, a->residual, a->pre, a->out, a->ld_res, a->act};
   const TilePlan tp = plan_tiles(s);
   const SlicePlan sp = plan_slices(s, A_MN);
-  if (sp.cost < tp.cost) {
-    constexpr auto kern = linear_slices_kernel<T, B_MN, A_MN>;
-    const int rc = more_shared_memory<kern>(s_smem(S_PIPE_ONE));
-    if (rc != HYC_OK) return rc;
-    SliceParams p;
-    p.s = s; p.e = e; p.tn = sp.tn; p.split = sp.split;
-    p.tiles_c = (s.C + 2 * BM - 1) / (2 * BM);
-    const int64_t ctas = 2ll * p.split * p.tiles_c * ((s.R + p.tn - 1) / p.tn);
-    const int pipe = ctas > num_sms() && p.tn <= 128 ? S_PIPE_TWO : S_PIPE_ONE;
-    p.stage_bytes = STAGE_A_BYTES + p.tn * BK;      // (tn / 2 rows of 128 bytes)
-    p.stages = pipe / p.stage_bytes < S_STAGES_MAX ? pipe / p.stage_bytes : S_STAGES_MAX;
-    p.tmem_cols = 32;
-    while (p.tmem_cols < p.tn) p.tmem_cols *= 2;
-    CUtensorMap mc, mr;
-    if (!operand_map(&mc, a->b, a->type, B_MN, s.C, s.K, a->ld_b, BM) || !operand_map(&mr, a->a, a->type, A_MN, s.R, s.K, a->ld_a, p.tn / 2))
-      return HYC_ERR_UNSUPPORTED;
-    return launch_cluster(kern, (unsigned)ctas, S_THREADS, (unsigned)(2 * p.split), s_smem(pipe), st, mc, mr, p);
-  }
+  if (sp.cost < tp.cost) return sp.pair ? launch_slices<T, A_MN, B_MN, true>(a, s, e, sp, st) : launch_slices<T, A_MN, B_MN, false>(a, s, e, sp, st);
   constexpr auto kern = linear_tiles_kernel<T, A_MN, B_MN>;
   const int rc = more_shared_memory<kern>(T_SMEM);
   if (rc != HYC_OK) return rc;
