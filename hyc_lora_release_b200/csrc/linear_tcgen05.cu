@@ -367,17 +367,16 @@ __device__ __forceinline__ void tc_ld16(uint32_t taddr, uint32_t (&v)[16]) {
 
 // the residual of 16 rows of the lane's column
 template <typename T>
-__device__ __forceinline__ void slice_residual(const SliceParams& p, int row0, int rows, int64_t col, float (&r)[16]) {
+__device__ __forceinline__ void slice_residual(const SliceParams& p, int row0, int rows, int64_t col, T (&r)[16]) {
   const T* res = (const T*)p.e.residual;
+  if (res == nullptr || col >= p.s.C) return;
 #pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    r[j] = 0.f;
-    if (res != nullptr && j < rows && col < p.s.C) r[j] = to_f32(res[(int64_t)(row0 + j) * p.e.ld_res + col]);
-  }
+  for (int j = 0; j < 16; ++j)
+    if (j < rows) r[j] = res[(int64_t)(row0 + j) * p.e.ld_res + col];
 }
 // 16 rows of results of the lane's column
 template <typename T>
-__device__ __forceinline__ void slice_block(const SliceParams& p, float (&v)[16], const float (&r)[16], float bias, int row0, int rows, int64_t col) {
+__device__ __forceinline__ void slice_block(const SliceParams& p, float (&v)[16], const T (&r)[16], float bias, int row0, int rows, int64_t col) {
   T *pre = (T*)p.e.pre, *out = (T*)p.e.out;
 #pragma unroll
   for (int j = 0; j < 16; ++j) v[j] += bias;
@@ -390,9 +389,13 @@ __device__ __forceinline__ void slice_block(const SliceParams& p, float (&v)[16]
 #pragma unroll
     for (int j = 0; j < 16; ++j) v[j] = act_of<decltype(a)::value>(v[j]);
   });
+  if (p.e.residual != nullptr) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] += to_f32(r[j]);
+  }
 #pragma unroll
   for (int j = 0; j < 16; ++j)
-    if (j < rows) out[(int64_t)(row0 + j) * p.s.C + col] = from_f32<T>(v[j] + r[j]);
+    if (j < rows) out[(int64_t)(row0 + j) * p.s.C + col] = from_f32<T>(v[j]);
 }
 
 // C_MN: the operand that gives the result's columns (B of the product) is MN-major; R_MN: the one that gives its rows (A).  PAIR: two CTAs
@@ -450,7 +453,8 @@ linear_slices_kernel(const __grid_constant__ CUtensorMap map_c, const __grid_con
   const uint32_t t_lane = tmem + ((uint32_t)(quad * 32) << 16);
   // the epilogue's blocks of 16 rows, dealt to the slices and their two groups of warps in turn
   const int end = min(p.s.R - r0, p.tn), first_row = 16 * (2 * slice + row_half), row_step = 32 * p.split;
-  float bias = 0.f, res[16];
+  float bias = 0.f;
+  T res[16];
   bool ok = true;
 
   if (warp == 0) {
@@ -521,7 +525,7 @@ linear_slices_kernel(const __grid_constant__ CUtensorMap map_c, const __grid_con
   if (p.split > 1) cluster_sync_all();
   if (warp >= 2 && ok) {
     for (int j0 = first_row; j0 < end; j0 += row_step) {
-      float now[16];
+      T now[16];
 #pragma unroll
       for (int j = 0; j < 16; ++j) now[j] = res[j];
       if (j0 + row_step < end) slice_residual<T>(p, r0 + j0 + row_step, end - j0 - row_step, col, res);
