@@ -46,27 +46,32 @@ struct QkParams {
   float* part;                     // backward: [blocks][d] sums of the weights' gradients, q's blocks first; or null
 };
 
-// The lane's channels of a head: NQ pairs of quads, o1 .. o1 + 3 and o2 .. o2 + 3
-template <int NQ> struct QkLane { int o1[NQ], o2[NQ]; bool live[NQ], turned[NQ]; };
-template <int NQ, int G>
-__device__ __forceinline__ QkLane<NQ> qk_lane(int li, int d, int half) {
-  QkLane<NQ> l;
+// The lane's channels of a head: NQ pairs of quads, from o1 and from o2 on.  FULL: the head's size is a power of two and all of it is
+// turned, so that every lane has channels, all of one kind, and partners at a distance known when this is compiled.
+template <int NQ, int G, bool FULL> struct QkLane {
+  int first[NQ], second[NQ];
+  bool is_live[NQ], is_turned[NQ];
+  __device__ __forceinline__ QkLane(int li, int d, int half) {
 #pragma unroll
-  for (int j = 0; j < NQ; ++j) {
-    const int at = li + j * G, i = at - half / 4;
-    l.live[j] = at < d / 8;
-    l.turned[j] = at < half / 4;
-    l.o1[j] = l.turned[j] ? 4 * at : 2 * half + 8 * i;
-    l.o2[j] = l.turned[j] ? 4 * at + half : 2 * half + 8 * i + 4;
-    if (!l.live[j]) { l.o1[j] = 0; l.o2[j] = 0; }
+    for (int j = 0; j < NQ; ++j) {
+      const int at = li + j * G, i = at - half / 4;
+      is_live[j] = at < d / 8;
+      is_turned[j] = at < half / 4;
+      first[j] = is_turned[j] ? 4 * at : 2 * half + 8 * i;
+      second[j] = is_turned[j] ? 4 * at + half : 2 * half + 8 * i + 4;
+      if (!is_live[j]) { first[j] = 0; second[j] = 0; }
+    }
   }
-  return l;
-}
+  __device__ __forceinline__ bool live(int j) const { return FULL || is_live[j]; }
+  __device__ __forceinline__ bool turned(int j) const { return FULL || is_turned[j]; }
+  __device__ __forceinline__ int o1(int j) const { return first[j]; }
+  __device__ __forceinline__ int o2(int j) const { return FULL ? first[j] + 4 * G * NQ : second[j]; }
+};
 
 // cos, sin and -sin of a token at the lane's channels; a position outside of the tables gives NaN, and reads nothing
 template <int NQ> struct QkAngles { f32x2 c[NQ][2], s[NQ][2], ns[NQ][2]; };
-template <int NQ>
-__device__ __forceinline__ void qk_angles(const QkParams& p, int b, int m, const QkLane<NQ>& l, QkAngles<NQ>& a) {
+template <int NQ, typename L>
+__device__ __forceinline__ void qk_angles(const QkParams& p, int b, int m, const L& l, QkAngles<NQ>& a) {
   int64_t at = m;
   if (p.pos != nullptr) {
     const int64_t i = b * p.pb + m * p.pm;
@@ -77,10 +82,10 @@ __device__ __forceinline__ void qk_angles(const QkParams& p, int b, int m, const
   for (int j = 0; j < NQ; ++j) {
     a.c[j][0] = a.c[j][1] = both(1.f);
     a.s[j][0] = a.s[j][1] = both(0.f);
-    if (l.turned[j]) {
+    if (l.turned(j)) {
       if (known) {
-        ld_any4(p.cos_t, at * p.ld_cos + l.o1[j], p.table_type, a.c[j]);
-        ld_any4(p.sin_t, at * p.ld_sin + l.o1[j], p.table_type, a.s[j]);
+        ld_any4(p.cos_t, at * p.ld_cos + l.o1(j), p.table_type, a.c[j]);
+        ld_any4(p.sin_t, at * p.ld_sin + l.o1(j), p.table_type, a.s[j]);
       } else {
         a.c[j][0] = a.c[j][1] = a.s[j][0] = a.s[j][1] = both(__int_as_float(0x7fc00000));
       }
@@ -112,7 +117,7 @@ __device__ __forceinline__ QkItem qk_item(const QkParams& p, const QkTensor& t, 
 }
 
 // UNROLL head groups are on their way at any time
-template <typename T, int G, int NQ, int UNROLL>
+template <typename T, int G, int NQ, bool FULL, int UNROLL>
 __global__ void __launch_bounds__(kQkThreads)
 qk_norm_fwd_kernel(const __grid_constant__ QkParams p) {
   pdl_wait();
@@ -121,12 +126,12 @@ qk_norm_fwd_kernel(const __grid_constant__ QkParams p) {
   const QkTensor& t = p.t[second ? 1 : 0];
   const int block = (int)blockIdx.x - (second ? p.t[0].blocks : 0);
   const int lane = threadIdx.x & 31, sub = lane / G;
-  const QkLane<NQ> l = qk_lane<NQ, G>(lane % G, p.d, p.half);
+  const QkLane<NQ, G, FULL> l(lane % G, p.d, p.half);
   f32x2 w1[NQ][2], w2[NQ][2];
 #pragma unroll
   for (int j = 0; j < NQ; ++j) {
-    ld_any4(t.w, l.o1[j], p.w_type, w1[j]);
-    ld_any4(t.w, l.o2[j], p.w_type, w2[j]);
+    ld_any4(t.w, l.o1(j), p.w_type, w1[j]);
+    ld_any4(t.w, l.o2(j), p.w_type, w2[j]);
   }
   const float inv_d = 1.f / (float)p.d;
   const uint32_t items = (uint32_t)p.tokens * (uint32_t)t.splits;
@@ -146,9 +151,9 @@ qk_norm_fwd_kernel(const __grid_constant__ QkParams p) {
     auto fetch = [&](int u, bool there) {
 #pragma unroll
       for (int j = 0; j < NQ; ++j)
-        if (l.live[j] && there) {
-          x1[u][j] = ld_quad(src + l.o1[j]);
-          x2[u][j] = ld_quad(src + l.o2[j]);
+        if (l.live(j) && there) {
+          x1[u][j] = ld_quad(src + l.o1(j));
+          x2[u][j] = ld_quad(src + l.o2(j));
         }
       src += step;
     };
@@ -165,7 +170,7 @@ qk_norm_fwd_kernel(const __grid_constant__ QkParams p) {
           f32x2 s = both(0.f);
 #pragma unroll
           for (int e = 0; e < 2; ++e) s = fma2f(f1[j][e], f1[j][e], fma2f(f2[j][e], f2[j][e], s));
-          if (l.live[j]) ss = add2f(ss, s);
+          if (l.live(j)) ss = add2f(ss, s);
         }
         fetch(u, left > (UNROLL + u) * PER);      // its place is free: the heads UNROLL groups on
         const float r = qk_rsqrt(fmaf(qk_sum<G>(qk_total(ss)), inv_d, p.eps));
@@ -179,9 +184,9 @@ qk_norm_fwd_kernel(const __grid_constant__ QkParams p) {
             y1[e] = fma2f(n2, a.ns[j][e], mul2f(n1, a.c[j][e]));
             y2[e] = fma2f(n1, a.s[j][e], mul2f(n2, a.c[j][e]));
           }
-          if (l.live[j] && left > u * PER) {
-            st_quad(dst + l.o1[j], y1);
-            st_quad(dst + l.o2[j], y2);
+          if (l.live(j) && left > u * PER) {
+            st_quad(dst + l.o1(j), y1);
+            st_quad(dst + l.o2(j), y2);
           }
         }
         dst += out_step;
@@ -190,7 +195,7 @@ qk_norm_fwd_kernel(const __grid_constant__ QkParams p) {
   }
 }
 
-template <typename T, int G, int NQ>
+template <typename T, int G, int NQ, bool FULL>
 __global__ void __launch_bounds__(kQkThreads, NQ == 1 ? kQkBwdBlocks : 1)
 qk_norm_bwd_kernel(const __grid_constant__ QkParams p) {
   __shared__ float s_part[kQkWarps][8 * G * NQ];
@@ -200,12 +205,12 @@ qk_norm_bwd_kernel(const __grid_constant__ QkParams p) {
   const QkTensor& t = p.t[second ? 1 : 0];
   const int block = (int)blockIdx.x - (second ? p.t[0].blocks : 0);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane / G;
-  const QkLane<NQ> l = qk_lane<NQ, G>(lane % G, p.d, p.half);
+  const QkLane<NQ, G, FULL> l(lane % G, p.d, p.half);
   f32x2 w1[NQ][2], w2[NQ][2], dw1[NQ][2], dw2[NQ][2];
 #pragma unroll
   for (int j = 0; j < NQ; ++j) {
-    ld_any4(t.w, l.o1[j], p.w_type, w1[j]);
-    ld_any4(t.w, l.o2[j], p.w_type, w2[j]);
+    ld_any4(t.w, l.o1(j), p.w_type, w1[j]);
+    ld_any4(t.w, l.o2(j), p.w_type, w2[j]);
     dw1[j][0] = dw1[j][1] = dw2[j][0] = dw2[j][1] = both(0.f);
   }
   const float inv_d = 1.f / (float)p.d;
@@ -226,9 +231,9 @@ qk_norm_bwd_kernel(const __grid_constant__ QkParams p) {
     auto fetch = [&](bool there) {
 #pragma unroll
       for (int j = 0; j < NQ; ++j)
-        if (l.live[j] && there) {
-          x1[j] = ld_quad(src + l.o1[j]); x2[j] = ld_quad(src + l.o2[j]);
-          d1[j] = ld_quad(grad + l.o1[j]); d2[j] = ld_quad(grad + l.o2[j]);
+        if (l.live(j) && there) {
+          x1[j] = ld_quad(src + l.o1(j)); x2[j] = ld_quad(src + l.o2(j));
+          d1[j] = ld_quad(grad + l.o1(j)); d2[j] = ld_quad(grad + l.o2(j));
         }
       src += step;
       grad += grad_step;
@@ -248,28 +253,30 @@ qk_norm_bwd_kernel(const __grid_constant__ QkParams p) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const f32x2 u = fma2f(g2[j][e], a.s[j][e], mul2f(g1[j][e], a.c[j][e])), v = fma2f(g1[j][e], a.ns[j][e], mul2f(g2[j][e], a.c[j][e]));
-          g1[j][e] = u; g2[j][e] = v;
           s1 = fma2f(f1[j][e], f1[j][e], fma2f(f2[j][e], f2[j][e], s1));
-          s2 = fma2f(mul2f(u, w1[j][e]), f1[j][e], fma2f(mul2f(v, w2[j][e]), f2[j][e], s2));
+          const f32x2 p1 = mul2f(u, f1[j][e]), p2 = mul2f(v, f2[j][e]);
+          s2 = fma2f(p1, w1[j][e], fma2f(p2, w2[j][e], s2));
+          g1[j][e] = u; g2[j][e] = v;
         }
-        if (l.live[j]) { ss = add2f(ss, s1); sg = add2f(sg, s2); }
+        if (l.live(j)) { ss = add2f(ss, s1); sg = add2f(sg, s2); }
       }
+      // dx = r g w - x r^2 mean(g w x r)
       const float r = qk_rsqrt(fmaf(qk_sum<G>(qk_total(ss)), inv_d, p.eps));
-      const float mean = qk_sum<G>(qk_total(sg)) * r * inv_d;
-      const f32x2 rr = both(r), nm = both(-mean);
+      const float pull = qk_sum<G>(qk_total(sg)) * (r * inv_d) * (r * -r);
+      const f32x2 rr = both(r), pp = both(pull);
 #pragma unroll
       for (int j = 0; j < NQ; ++j) {
         f32x2 y1[2], y2[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const f32x2 n1 = mul2f(f1[j][e], rr), n2 = mul2f(f2[j][e], rr);
-          if (ok) { dw1[j][e] = fma2f(g1[j][e], n1, dw1[j][e]); dw2[j][e] = fma2f(g2[j][e], n2, dw2[j][e]); }
-          y1[e] = mul2f(rr, fma2f(n1, nm, mul2f(g1[j][e], w1[j][e])));
-          y2[e] = mul2f(rr, fma2f(n2, nm, mul2f(g2[j][e], w2[j][e])));
+          const f32x2 u = mul2f(g1[j][e], rr), v = mul2f(g2[j][e], rr);
+          if (ok) { dw1[j][e] = fma2f(u, f1[j][e], dw1[j][e]); dw2[j][e] = fma2f(v, f2[j][e], dw2[j][e]); }
+          y1[e] = fma2f(f1[j][e], pp, mul2f(u, w1[j][e]));
+          y2[e] = fma2f(f2[j][e], pp, mul2f(v, w2[j][e]));
         }
-        if (ok && l.live[j]) {
-          st_quad(dst + l.o1[j], y1);
-          st_quad(dst + l.o2[j], y2);
+        if (ok && l.live(j)) {
+          st_quad(dst + l.o1(j), y1);
+          st_quad(dst + l.o2(j), y2);
         }
       }
       dst += out_step;
@@ -285,10 +292,10 @@ qk_norm_bwd_kernel(const __grid_constant__ QkParams p) {
         dw1[j][e] = add2f(dw1[j][e], __shfl_xor_sync(0xffffffffu, (unsigned long long)dw1[j][e], o));
         dw2[j][e] = add2f(dw2[j][e], __shfl_xor_sync(0xffffffffu, (unsigned long long)dw2[j][e], o));
       }
-      if (sub == 0 && l.live[j]) {
+      if (sub == 0 && l.live(j)) {
         const float2 u = unpair(dw1[j][e]), v = unpair(dw2[j][e]);
-        s_part[warp][l.o1[j] + 2 * e] = u.x; s_part[warp][l.o1[j] + 2 * e + 1] = u.y;
-        s_part[warp][l.o2[j] + 2 * e] = v.x; s_part[warp][l.o2[j] + 2 * e + 1] = v.y;
+        s_part[warp][l.o1(j) + 2 * e] = u.x; s_part[warp][l.o1(j) + 2 * e + 1] = u.y;
+        s_part[warp][l.o2(j) + 2 * e] = v.x; s_part[warp][l.o2(j) + 2 * e + 1] = v.y;
       }
     }
   __syncthreads();
@@ -392,18 +399,22 @@ static void qk_fill(QkParams& p, const hyc_qk_norm* a) {
   p.part = nullptr;
 }
 
-// f(element, lanes of a head, pairs of quads per lane)
+// f(element, lanes of a head, pairs of quads per lane, FULL)
 template <typename F>
-static int qk_by_type(int type, int d, F&& f) {
+static int qk_by_type(int type, int d, int rot, F&& f) {
   auto by_group = [&](auto elem) -> int {
     using std::integral_constant;
+    auto full = [&](auto group, auto quads) -> int {
+      if (rot == d && d == 8 * decltype(group)::value * decltype(quads)::value) return f(elem, group, quads, std::true_type());
+      return f(elem, group, quads, std::false_type());
+    };
     constexpr integral_constant<int, 1> one{};
     switch (qk_group(d)) {
-      case 2: return f(elem, integral_constant<int, 2>(), one);
-      case 4: return f(elem, integral_constant<int, 4>(), one);
-      case 8: return f(elem, integral_constant<int, 8>(), one);
-      case 16: return f(elem, integral_constant<int, 16>(), one);
-      default: return d <= 256 ? f(elem, integral_constant<int, 32>(), one) : f(elem, integral_constant<int, 32>(), integral_constant<int, 2>());
+      case 2: return full(integral_constant<int, 2>(), one);
+      case 4: return full(integral_constant<int, 4>(), one);
+      case 8: return full(integral_constant<int, 8>(), one);
+      case 16: return full(integral_constant<int, 16>(), one);
+      default: return d <= 256 ? full(integral_constant<int, 32>(), one) : full(integral_constant<int, 32>(), integral_constant<int, 2>());
     }
   };
   if (type == HYC_F32) return by_group(float());
@@ -420,8 +431,8 @@ extern "C" HYC_API int hyc_qk_norm_rope_fwd(const hyc_qk_norm* a, void* stream) 
   if (rc != HYC_OK || a->batch * a->seq == 0) return rc;
   QkParams p;
   qk_fill(p, a);
-  return qk_by_type(a->type, p.d, [&](auto elem, auto group, auto quads) -> int {
-    auto kern = qk_norm_fwd_kernel<decltype(elem), decltype(group)::value, decltype(quads)::value, 2>;
+  return qk_by_type(a->type, p.d, 2 * p.half, [&](auto elem, auto group, auto quads, auto full) -> int {
+    auto kern = qk_norm_fwd_kernel<decltype(elem), decltype(group)::value, decltype(quads)::value, decltype(full)::value, 2>;
     qk_plan(p, num_sms() * resident_blocks(kern, kQkThreads, 0, 2));
     launch_pdl(kern, dim3((unsigned)(p.t[0].blocks + p.t[1].blocks)), dim3(kQkThreads), 0, (cudaStream_t)stream, p);
     HYC_CHECK_LAUNCH();
@@ -444,8 +455,8 @@ extern "C" HYC_API int hyc_qk_norm_rope_bwd(const hyc_qk_norm* a, void* dweight_
   qk_fill(p, a);
   if (p.tokens > 0) {
     p.part = weights ? (float*)workspace : nullptr;
-    const int r = qk_by_type(a->type, p.d, [&](auto elem, auto group, auto quads) -> int {
-      auto kern = qk_norm_bwd_kernel<decltype(elem), decltype(group)::value, decltype(quads)::value>;
+    const int r = qk_by_type(a->type, p.d, 2 * p.half, [&](auto elem, auto group, auto quads, auto full) -> int {
+      auto kern = qk_norm_bwd_kernel<decltype(elem), decltype(group)::value, decltype(quads)::value, decltype(full)::value>;
       const int res = resident_blocks(kern, kQkThreads, 0, 1);
       qk_plan(p, num_sms() * (res < kQkBwdBlocks ? res : kQkBwdBlocks));
       launch_pdl(kern, dim3((unsigned)(p.t[0].blocks + p.t[1].blocks)), dim3(kQkThreads), 0, (cudaStream_t)stream, p);
