@@ -98,43 +98,35 @@ __device__ __forceinline__ f32x2 add2f(f32x2 a, f32x2 b) { f32x2 r; asm("add.rn.
 __device__ __forceinline__ f32x2 mul2f(f32x2 a, f32x2 b) { f32x2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
 __device__ __forceinline__ f32x2 fma2f(f32x2 a, f32x2 b, f32x2 c) { f32x2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
 
-// four adjacent values as two pairs: 8 bytes of 16-bit elements, 16 of fp32
-template <typename T> struct Quad { uint2 v; };
-template <> struct Quad<float> { uint4 v; };
-template <typename T> __device__ __forceinline__ Quad<T> ld_quad(const T* p) {
-  Quad<T> q;
-  q.v = *reinterpret_cast<const decltype(q.v)*>(p);
-  return q;
+// eight adjacent values as four pairs
+__device__ __forceinline__ void octet_to_pairs(const Octet<__nv_bfloat16>& o, f32x2 (&f)[4]) {
+  const uint32_t w[4] = {o.v[0].x, o.v[0].y, o.v[0].z, o.v[0].w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = pair(bf16lo_to_f32(w[i]), bf16hi_to_f32(w[i]));
 }
-__device__ __forceinline__ void quad_to_f32(const Quad<__nv_bfloat16>& q, f32x2 (&f)[2]) {
-  f[0] = pair(bf16lo_to_f32(q.v.x), bf16hi_to_f32(q.v.x));
-  f[1] = pair(bf16lo_to_f32(q.v.y), bf16hi_to_f32(q.v.y));
+__device__ __forceinline__ void octet_to_pairs(const Octet<__half>& o, f32x2 (&f)[4]) {
+  const uint32_t w[4] = {o.v[0].x, o.v[0].y, o.v[0].z, o.v[0].w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { const float2 t = half2_bits_to_f32(w[i]); f[i] = pair(t.x, t.y); }
 }
-__device__ __forceinline__ void quad_to_f32(const Quad<__half>& q, f32x2 (&f)[2]) {
-  const float2 a = half2_bits_to_f32(q.v.x), b = half2_bits_to_f32(q.v.y);
-  f[0] = pair(a.x, a.y);
-  f[1] = pair(b.x, b.y);
+__device__ __forceinline__ void octet_to_pairs(const Octet<float>& o, f32x2 (&f)[4]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    f[2 * i] = pair(__uint_as_float(o.v[i].x), __uint_as_float(o.v[i].y));
+    f[2 * i + 1] = pair(__uint_as_float(o.v[i].z), __uint_as_float(o.v[i].w));
+  }
 }
-__device__ __forceinline__ void quad_to_f32(const Quad<float>& q, f32x2 (&f)[2]) {
-  f[0] = pair(__uint_as_float(q.v.x), __uint_as_float(q.v.y));
-  f[1] = pair(__uint_as_float(q.v.z), __uint_as_float(q.v.w));
+template <typename T>
+__device__ __forceinline__ void st_pairs(T* p, const f32x2 (&f)[4]) {
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { const float2 t = unpair(f[i]); v[2 * i] = t.x; v[2 * i + 1] = t.y; }
+  st_octet(p, v);
 }
-__device__ __forceinline__ void st_quad(__nv_bfloat16* p, const f32x2 (&f)[2]) {
-  const float2 a = unpair(f[0]), b = unpair(f[1]);
-  *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2_rn(a.x, a.y), pack_bf16x2_rn(b.x, b.y));
-}
-__device__ __forceinline__ void st_quad(__half* p, const f32x2 (&f)[2]) {
-  const float2 a = unpair(f[0]), b = unpair(f[1]);
-  *reinterpret_cast<uint2*>(p) = make_uint2(f32_to_half2_bits(a.x, a.y), f32_to_half2_bits(b.x, b.y));
-}
-__device__ __forceinline__ void st_quad(float* p, const f32x2 (&f)[2]) {
-  const float2 a = unpair(f[0]), b = unpair(f[1]);
-  *reinterpret_cast<float4*>(p) = make_float4(a.x, a.y, b.x, b.y);
-}
-__device__ __forceinline__ void ld_any4(const void* p, int64_t at, int type, f32x2 (&f)[2]) {
-  if (type == HYC_F32) quad_to_f32(ld_quad(reinterpret_cast<const float*>(p) + at), f);
-  else if (type == HYC_F16) quad_to_f32(ld_quad(reinterpret_cast<const __half*>(p) + at), f);
-  else quad_to_f32(ld_quad(reinterpret_cast<const __nv_bfloat16*>(p) + at), f);
+__device__ __forceinline__ void ld_any_pairs(const void* p, int64_t at, int type, f32x2 (&f)[4]) {
+  if (type == HYC_F32) octet_to_pairs(ld_octet(reinterpret_cast<const float*>(p) + at), f);
+  else if (type == HYC_F16) octet_to_pairs(ld_octet(reinterpret_cast<const __half*>(p) + at), f);
+  else octet_to_pairs(ld_octet(reinterpret_cast<const __nv_bfloat16*>(p) + at), f);
 }
 
 inline bool elem_type_ok(int t) { return t == HYC_BF16 || t == HYC_F16 || t == HYC_F32; }

@@ -52,6 +52,20 @@ inline int resident_blocks(K kern, int threads, size_t smem, int otherwise) {
   return n;
 }
 
+// Lets a kernel have up to `bytes` of dynamic shared memory, the same number on every call: said once per kernel and device.
+template <auto KERN>
+inline int more_shared_memory(int bytes) {
+  static bool done[64] = {false};      // (the attribute belongs to a function and a device)
+  const int slot = current_device_slot();
+  if (bytes <= 49152 || (slot >= 0 && done[slot])) return HYC_OK;
+  if (cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
+    hyc_set_last_cuda_error((int)cudaGetLastError());
+    return HYC_ERR_LAUNCH;
+  }
+  if (slot >= 0) done[slot] = true;
+  return HYC_OK;
+}
+
 // Programmatic dependent launch: a kernel launched with launch_pdl (GEMMs and kernels in clusters set the attribute in launch code
 // of their own) may begin before the kernel in front of it in the stream has ended, and has to call pdl_wait() before it touches
 // global memory (pdl_wait returns once that kernel is complete and its writes are visible; since every such kernel waits, so is

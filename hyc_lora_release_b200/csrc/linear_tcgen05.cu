@@ -635,19 +635,6 @@ static bool operand_map(CUtensorMap* m, const void* ptr, int type, bool mn, int6
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <auto KERN>
-static int more_shared_memory(int bytes) {
-  static bool done[64] = {false};      // (the attribute belongs to a function and a device)
-  const int slot = current_device_slot();
-  if (slot >= 0 && done[slot]) return HYC_OK;
-  if (cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
-    hyc_set_last_cuda_error((int)cudaGetLastError());
-    return HYC_ERR_LAUNCH;
-  }
-  if (slot >= 0) done[slot] = true;
-  return HYC_OK;
-}
-
 template <typename K, typename... A>
 static int launch_cluster(K kern, unsigned blocks, unsigned threads, unsigned cluster, int smem, cudaStream_t st, const A&... args) {
   cudaLaunchConfig_t cfg = {};

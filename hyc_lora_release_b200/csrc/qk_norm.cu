@@ -19,7 +19,7 @@
 namespace hyc {
 
 constexpr int kQkThreads = 256, kQkWarps = kQkThreads / 32;
-constexpr int kQkBwdBlocks = 3;      // blocks per SM that backward's registers are cut for and its workspace counts on
+constexpr int kQkBwdBlocks = 2;      // blocks per SM that backward's registers are cut for and its workspace counts on
 
 // one instruction, two units in the last place (the root and the quotient, each rounded, take two dozen per head)
 __device__ __forceinline__ float qk_rsqrt(float v) {
@@ -46,32 +46,29 @@ struct QkParams {
   float* part;                     // backward: [blocks][d] sums of the weights' gradients, q's blocks first; or null
 };
 
-// The lane's channels of a head: NQ pairs of quads, from o1 and from o2 on.  FULL: the head's size is a power of two and all of it is
+// The lane's channels of a head: the octets from o1 and from o2 on.  FULL: the head's size is 16 times a power of two and all of it is
 // turned, so that every lane has channels, all of one kind, and partners at a distance known when this is compiled.
-template <int NQ, int G, bool FULL> struct QkLane {
-  int first[NQ], second[NQ];
-  bool is_live[NQ], is_turned[NQ];
+template <int G, bool FULL> struct QkLane {
+  int first, second;
+  bool is_live, is_turned;
   __device__ __forceinline__ QkLane(int li, int d, int half) {
-#pragma unroll
-    for (int j = 0; j < NQ; ++j) {
-      const int at = li + j * G, i = at - half / 4;
-      is_live[j] = at < d / 8;
-      is_turned[j] = at < half / 4;
-      first[j] = is_turned[j] ? 4 * at : 2 * half + 8 * i;
-      second[j] = is_turned[j] ? 4 * at + half : 2 * half + 8 * i + 4;
-      if (!is_live[j]) { first[j] = 0; second[j] = 0; }
-    }
+    const int i = li - half / 8;
+    is_live = li < d / 16;
+    is_turned = li < half / 8;
+    first = is_turned ? 8 * li : 2 * half + 16 * i;
+    second = is_turned ? 8 * li + half : 2 * half + 16 * i + 8;
+    if (!is_live) { first = 0; second = 0; }
   }
-  __device__ __forceinline__ bool live(int j) const { return FULL || is_live[j]; }
-  __device__ __forceinline__ bool turned(int j) const { return FULL || is_turned[j]; }
-  __device__ __forceinline__ int o1(int j) const { return first[j]; }
-  __device__ __forceinline__ int o2(int j) const { return FULL ? first[j] + 4 * G * NQ : second[j]; }
+  __device__ __forceinline__ bool live() const { return FULL || is_live; }
+  __device__ __forceinline__ bool turned() const { return FULL || is_turned; }
+  __device__ __forceinline__ int o1() const { return first; }
+  __device__ __forceinline__ int o2() const { return FULL ? first + 8 * G : second; }
 };
 
 // cos, sin and -sin of a token at the lane's channels; a position outside of the tables gives NaN, and reads nothing
-template <int NQ> struct QkAngles { f32x2 c[NQ][2], s[NQ][2], ns[NQ][2]; };
-template <int NQ, typename L>
-__device__ __forceinline__ void qk_angles(const QkParams& p, int b, int m, const L& l, QkAngles<NQ>& a) {
+struct QkAngles { f32x2 c[4], s[4], ns[4]; };
+template <typename L>
+__device__ __forceinline__ void qk_angles(const QkParams& p, int b, int m, const L& l, QkAngles& a) {
   int64_t at = m;
   if (p.pos != nullptr) {
     const int64_t i = b * p.pb + m * p.pm;
@@ -79,20 +76,16 @@ __device__ __forceinline__ void qk_angles(const QkParams& p, int b, int m, const
   }
   const bool known = at >= 0 && at < p.table_rows;
 #pragma unroll
-  for (int j = 0; j < NQ; ++j) {
-    a.c[j][0] = a.c[j][1] = both(1.f);
-    a.s[j][0] = a.s[j][1] = both(0.f);
-    if (l.turned(j)) {
-      if (known) {
-        ld_any4(p.cos_t, at * p.ld_cos + l.o1(j), p.table_type, a.c[j]);
-        ld_any4(p.sin_t, at * p.ld_sin + l.o1(j), p.table_type, a.s[j]);
-      } else {
-        a.c[j][0] = a.c[j][1] = a.s[j][0] = a.s[j][1] = both(__int_as_float(0x7fc00000));
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < 2; ++e) a.ns[j][e] = a.s[j][e] ^ 0x8000000080000000ull;
+  for (int e = 0; e < 4; ++e) {
+    a.c[e] = both(known || !l.turned() ? 1.f : __int_as_float(0x7fc00000));
+    a.s[e] = both(known || !l.turned() ? 0.f : __int_as_float(0x7fc00000));
   }
+  if (l.turned() && known) {
+    ld_any_pairs(p.cos_t, at * p.ld_cos + l.o1(), p.table_type, a.c);
+    ld_any_pairs(p.sin_t, at * p.ld_sin + l.o1(), p.table_type, a.s);
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) a.ns[e] = a.s[e] ^ 0x8000000080000000ull;
 }
 
 template <int G>
@@ -116,193 +109,214 @@ __device__ __forceinline__ QkItem qk_item(const QkParams& p, const QkTensor& t, 
   return i;
 }
 
-// UNROLL head groups are on their way at any time
-template <typename T, int G, int NQ, bool FULL, int UNROLL>
-__global__ void __launch_bounds__(kQkThreads)
+// ---- a warp's head groups, those of all its items in a row, on their way into shared memory kQkRing at a time: every lane copies the
+// octets that it will read itself, so that nobody waits for another lane
+constexpr int kQkRing = 4;
+__device__ __forceinline__ void qk_copy(uint32_t to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+// PER: heads of a warp at a time; BWD: x and dy, else x
+template <typename T, int PER, bool BWD, typename L>
+struct QkFeed {
+  static constexpr int OCTETS = BWD ? 4 : 2, PARTS = (int)sizeof(T) / 2, STRIDE = kQkThreads * 16;      // 16-byte parts of an octet; of the block's lanes
+  static constexpr int PLACE = OCTETS * PARTS * STRIDE;
+  const QkParams& p;
+  const QkTensor& t;
+  const L& l;
+  const T *src, *grad;
+  int64_t step, grad_step;
+  uint32_t item, items, item_step, base, put, got, top;
+  int left, sub;
+  __device__ __forceinline__ QkFeed(const QkParams& p_, const QkTensor& t_, const L& l_, uint32_t first, uint32_t items_, uint32_t item_step_, int sub_, uint32_t smem)
+      : p(p_), t(t_), l(l_), step(PER * t_.xh), grad_step(BWD ? PER * t_.gh : 0), item(first), items(items_), item_step(item_step_),
+        base(smem + threadIdx.x * 16), put(base), got(base), top(base + kQkRing * PLACE), sub(sub_) {
+    open();
+#pragma unroll
+    for (int i = 0; i < kQkRing - 1; ++i) send();
+  }
+  __device__ __forceinline__ void open() {
+    if (item >= items) return;
+    const QkItem it = qk_item(p, t, item);
+    const int head0 = it.first * PER + sub;
+    left = min((it.first + t.per_split) * PER, t.heads) - head0;
+    src = reinterpret_cast<const T*>(t.x) + it.b * t.xb + it.m * t.xm + head0 * t.xh;
+    if (BWD) grad = reinterpret_cast<const T*>(t.dy) + it.b * t.gb + it.m * t.gm + head0 * t.gh;
+  }
+  __device__ __forceinline__ void copy(int octet, const T* from) {
+#pragma unroll
+    for (int i = 0; i < PARTS; ++i) qk_copy(put + (uint32_t)((octet * PARTS + i) * STRIDE), from + i * (16 / (int)sizeof(T)));
+  }
+  // the next group's copies, into the ring's next place (nothing once all are under way: the groups stay countable)
+  __device__ __forceinline__ void send() {
+    if (item < items) {
+      if (l.live() && left > 0) {
+        copy(0, src + l.o1());
+        copy(1, src + l.o2());
+        if (BWD) {
+          copy(2, grad + l.o1());
+          copy(3, grad + l.o2());
+        }
+      }
+      src += step;
+      if (BWD) grad += grad_step;
+      left -= PER;
+      if (left <= -sub) { item += item_step; open(); }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    put += PLACE;
+    if (put == top) put = base;
+  }
+  __device__ __forceinline__ void wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kQkRing - 2) : "memory"); }
+  __device__ __forceinline__ void take(int octet, f32x2 (&f)[4]) const {
+    Octet<T> o;
+#pragma unroll
+    for (int i = 0; i < PARTS; ++i)
+      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(o.v[i].x), "=r"(o.v[i].y), "=r"(o.v[i].z), "=r"(o.v[i].w) : "r"(got + (uint32_t)((octet * PARTS + i) * STRIDE)) : "memory");
+    octet_to_pairs(o, f);
+  }
+  __device__ __forceinline__ void next() {
+    got += PLACE;
+    if (got == top) got = base;
+  }
+};
+
+template <typename T, int G, bool FULL>
+__global__ void __launch_bounds__(kQkThreads, 3)
 qk_norm_fwd_kernel(const __grid_constant__ QkParams p) {
+  extern __shared__ __align__(16) uint8_t s_ring[];
   pdl_wait();
   constexpr int PER = 32 / G;      // heads of a warp at a time
   const bool second = (int)blockIdx.x >= p.t[0].blocks;
   const QkTensor& t = p.t[second ? 1 : 0];
   const int block = (int)blockIdx.x - (second ? p.t[0].blocks : 0);
   const int lane = threadIdx.x & 31, sub = lane / G;
-  const QkLane<NQ, G, FULL> l(lane % G, p.d, p.half);
-  f32x2 w1[NQ][2], w2[NQ][2];
-#pragma unroll
-  for (int j = 0; j < NQ; ++j) {
-    ld_any4(t.w, l.o1(j), p.w_type, w1[j]);
-    ld_any4(t.w, l.o2(j), p.w_type, w2[j]);
-  }
+  typedef QkLane<G, FULL> Lane;
+  const Lane l(lane % G, p.d, p.half);
+  const uint32_t items = (uint32_t)p.tokens * (uint32_t)t.splits, item_step = (uint32_t)t.blocks * kQkWarps;
+  const uint32_t first = (uint32_t)block * kQkWarps + (threadIdx.x >> 5);
+  QkFeed<T, PER, false, Lane> feed(p, t, l, first, items, item_step, sub, (uint32_t)__cvta_generic_to_shared(s_ring));
+  f32x2 w1[4], w2[4];
+  ld_any_pairs(t.w, l.o1(), p.w_type, w1);
+  ld_any_pairs(t.w, l.o2(), p.w_type, w2);
   const float inv_d = 1.f / (float)p.d;
-  const uint32_t items = (uint32_t)p.tokens * (uint32_t)t.splits;
-  for (uint32_t item = (uint32_t)block * kQkWarps + (threadIdx.x >> 5); item < items; item += (uint32_t)t.blocks * kQkWarps) {
+  const int out_step = PER * p.d;
+  for (uint32_t item = first; item < items; item += item_step) {
     const QkItem it = qk_item(p, t, item);
-    const T* xt = reinterpret_cast<const T*>(t.x) + it.b * t.xb + it.m * t.xm;
-    T* ot = reinterpret_cast<T*>(t.out) + (int64_t)it.token * t.heads * p.d;
-    QkAngles<NQ> a;
-    qk_angles<NQ>(p, it.b, it.m, l, a);
+    QkAngles a;
+    qk_angles(p, it.b, it.m, l, a);
     const int head0 = it.first * PER + sub;
-    int left = min((it.first + t.per_split) * PER, t.heads) - head0;      // heads of this lane's kind: left > u PER
-    const T* src = xt + head0 * t.xh;
-    T* dst = ot + head0 * p.d;
-    const int64_t step = PER * t.xh;
-    const int out_step = PER * p.d;
-    Quad<T> x1[UNROLL][NQ], x2[UNROLL][NQ];
-    auto fetch = [&](int u, bool there) {
+    int left = min((it.first + t.per_split) * PER, t.heads) - head0;
+    T* dst = reinterpret_cast<T*>(t.out) + (int64_t)it.token * t.heads * p.d + head0 * p.d + l.o1();
+    for (; left > -sub; left -= PER, dst += out_step) {
+      f32x2 f1[4], f2[4], ss = both(0.f);
+      feed.wait();
+      feed.take(0, f1);
+      feed.take(1, f2);
+      feed.next();
+      feed.send();
 #pragma unroll
-      for (int j = 0; j < NQ; ++j)
-        if (l.live(j) && there) {
-          x1[u][j] = ld_quad(src + l.o1(j));
-          x2[u][j] = ld_quad(src + l.o2(j));
-        }
-      src += step;
-    };
+      for (int e = 0; e < 4; ++e) ss = fma2f(f1[e], f1[e], fma2f(f2[e], f2[e], ss));
+      const f32x2 rr = both(qk_rsqrt(fmaf(qk_sum<G>(l.live() ? qk_total(ss) : 0.f), inv_d, p.eps)));
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) fetch(u, left > u * PER);
-    for (; left > -sub; left -= UNROLL * PER) {
-#pragma unroll
-      for (int u = 0; u < UNROLL; ++u) {
-        f32x2 f1[NQ][2], f2[NQ][2], ss = both(0.f);
-#pragma unroll
-        for (int j = 0; j < NQ; ++j) {
-          quad_to_f32(x1[u][j], f1[j]);
-          quad_to_f32(x2[u][j], f2[j]);
-          f32x2 s = both(0.f);
-#pragma unroll
-          for (int e = 0; e < 2; ++e) s = fma2f(f1[j][e], f1[j][e], fma2f(f2[j][e], f2[j][e], s));
-          if (l.live(j)) ss = add2f(ss, s);
-        }
-        fetch(u, left > (UNROLL + u) * PER);      // its place is free: the heads UNROLL groups on
-        const float r = qk_rsqrt(fmaf(qk_sum<G>(qk_total(ss)), inv_d, p.eps));
-        const f32x2 rr = both(r);
-#pragma unroll
-        for (int j = 0; j < NQ; ++j) {
-          f32x2 y1[2], y2[2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const f32x2 n1 = mul2f(mul2f(f1[j][e], rr), w1[j][e]), n2 = mul2f(mul2f(f2[j][e], rr), w2[j][e]);
-            y1[e] = fma2f(n2, a.ns[j][e], mul2f(n1, a.c[j][e]));
-            y2[e] = fma2f(n1, a.s[j][e], mul2f(n2, a.c[j][e]));
-          }
-          if (l.live(j) && left > u * PER) {
-            st_quad(dst + l.o1(j), y1);
-            st_quad(dst + l.o2(j), y2);
-          }
-        }
-        dst += out_step;
+      for (int e = 0; e < 4; ++e) {
+        const f32x2 n1 = mul2f(mul2f(f1[e], rr), w1[e]), n2 = mul2f(mul2f(f2[e], rr), w2[e]);
+        f1[e] = fma2f(n2, a.ns[e], mul2f(n1, a.c[e]));
+        f2[e] = fma2f(n1, a.s[e], mul2f(n2, a.c[e]));
+      }
+      if (l.live() && left > 0) {
+        st_pairs(dst, f1);
+        st_pairs(dst + (l.o2() - l.o1()), f2);
       }
     }
   }
 }
 
-template <typename T, int G, int NQ, bool FULL>
-__global__ void __launch_bounds__(kQkThreads, NQ == 1 ? kQkBwdBlocks : 1)
+template <typename T, int G, bool FULL>
+__global__ void __launch_bounds__(kQkThreads, kQkBwdBlocks)
 qk_norm_bwd_kernel(const __grid_constant__ QkParams p) {
-  __shared__ float s_part[kQkWarps][8 * G * NQ];
+  extern __shared__ __align__(16) uint8_t s_ring[];
   pdl_wait();
   constexpr int PER = 32 / G;
   const bool second = (int)blockIdx.x >= p.t[0].blocks;
   const QkTensor& t = p.t[second ? 1 : 0];
   const int block = (int)blockIdx.x - (second ? p.t[0].blocks : 0);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane / G;
-  const QkLane<NQ, G, FULL> l(lane % G, p.d, p.half);
-  f32x2 w1[NQ][2], w2[NQ][2], dw1[NQ][2], dw2[NQ][2];
+  typedef QkLane<G, FULL> Lane;
+  const Lane l(lane % G, p.d, p.half);
+  const uint32_t items = (uint32_t)p.tokens * (uint32_t)t.splits, item_step = (uint32_t)t.blocks * kQkWarps;
+  const uint32_t first = (uint32_t)block * kQkWarps + (uint32_t)warp;
+  QkFeed<T, PER, true, Lane> feed(p, t, l, first, items, item_step, sub, (uint32_t)__cvta_generic_to_shared(s_ring));
+  f32x2 w1[4], w2[4], dw1[4], dw2[4];
+  ld_any_pairs(t.w, l.o1(), p.w_type, w1);
+  ld_any_pairs(t.w, l.o2(), p.w_type, w2);
 #pragma unroll
-  for (int j = 0; j < NQ; ++j) {
-    ld_any4(t.w, l.o1(j), p.w_type, w1[j]);
-    ld_any4(t.w, l.o2(j), p.w_type, w2[j]);
-    dw1[j][0] = dw1[j][1] = dw2[j][0] = dw2[j][1] = both(0.f);
-  }
+  for (int e = 0; e < 4; ++e) dw1[e] = dw2[e] = both(0.f);
   const float inv_d = 1.f / (float)p.d;
-  const uint32_t items = (uint32_t)p.tokens * (uint32_t)t.splits;
-  for (uint32_t item = (uint32_t)block * kQkWarps + warp; item < items; item += (uint32_t)t.blocks * kQkWarps) {
+  const int out_step = PER * p.d;
+  for (uint32_t item = first; item < items; item += item_step) {
     const QkItem it = qk_item(p, t, item);
-    const T *xt = reinterpret_cast<const T*>(t.x) + it.b * t.xb + it.m * t.xm, *gt = reinterpret_cast<const T*>(t.dy) + it.b * t.gb + it.m * t.gm;
-    T* ot = reinterpret_cast<T*>(t.out) + (int64_t)it.token * t.heads * p.d;
-    QkAngles<NQ> a;
-    qk_angles<NQ>(p, it.b, it.m, l, a);
+    QkAngles a;
+    qk_angles(p, it.b, it.m, l, a);
     const int head0 = it.first * PER + sub;
     int left = min((it.first + t.per_split) * PER, t.heads) - head0;
-    const T *src = xt + head0 * t.xh, *grad = gt + head0 * t.gh;
-    T* dst = ot + head0 * p.d;
-    const int64_t step = PER * t.xh, grad_step = PER * t.gh;
-    const int out_step = PER * p.d;
-    Quad<T> x1[NQ], x2[NQ], d1[NQ], d2[NQ];
-    auto fetch = [&](bool there) {
-#pragma unroll
-      for (int j = 0; j < NQ; ++j)
-        if (l.live(j) && there) {
-          x1[j] = ld_quad(src + l.o1(j)); x2[j] = ld_quad(src + l.o2(j));
-          d1[j] = ld_quad(grad + l.o1(j)); d2[j] = ld_quad(grad + l.o2(j));
-        }
-      src += step;
-      grad += grad_step;
-    };
-    fetch(left > 0);
-    for (; left > -sub; left -= PER) {
+    T* dst = reinterpret_cast<T*>(t.out) + (int64_t)it.token * t.heads * p.d + head0 * p.d + l.o1();
+    for (; left > -sub; left -= PER, dst += out_step) {
       const bool ok = left > 0;
-      f32x2 f1[NQ][2], f2[NQ][2], g1[NQ][2], g2[NQ][2], ss = both(0.f), sg = both(0.f);
+      f32x2 f1[4], f2[4], g1[4], g2[4], ss = both(0.f), sg = both(0.f);
+      feed.wait();
+      feed.take(0, f1);
+      feed.take(1, f2);
+      feed.take(2, g1);
+      feed.take(3, g2);
+      feed.next();
+      feed.send();
 #pragma unroll
-      for (int j = 0; j < NQ; ++j) {
-        quad_to_f32(x1[j], f1[j]); quad_to_f32(x2[j], f2[j]); quad_to_f32(d1[j], g1[j]); quad_to_f32(d2[j], g2[j]);
-      }
-      fetch(left > PER);      // the next heads while these are computed
-#pragma unroll
-      for (int j = 0; j < NQ; ++j) {
-        f32x2 s1 = both(0.f), s2 = both(0.f);
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const f32x2 u = fma2f(g2[j][e], a.s[j][e], mul2f(g1[j][e], a.c[j][e])), v = fma2f(g1[j][e], a.ns[j][e], mul2f(g2[j][e], a.c[j][e]));
-          s1 = fma2f(f1[j][e], f1[j][e], fma2f(f2[j][e], f2[j][e], s1));
-          const f32x2 p1 = mul2f(u, f1[j][e]), p2 = mul2f(v, f2[j][e]);
-          s2 = fma2f(p1, w1[j][e], fma2f(p2, w2[j][e], s2));
-          g1[j][e] = u; g2[j][e] = v;
-        }
-        if (l.live(j)) { ss = add2f(ss, s1); sg = add2f(sg, s2); }
+      for (int e = 0; e < 4; ++e) {
+        const f32x2 u = fma2f(g2[e], a.s[e], mul2f(g1[e], a.c[e])), v = fma2f(g1[e], a.ns[e], mul2f(g2[e], a.c[e]));
+        ss = fma2f(f1[e], f1[e], fma2f(f2[e], f2[e], ss));
+        sg = fma2f(mul2f(u, f1[e]), w1[e], fma2f(mul2f(v, f2[e]), w2[e], sg));
+        g1[e] = u; g2[e] = v;
       }
       // dx = r g w - x r^2 mean(g w x r)
-      const float r = qk_rsqrt(fmaf(qk_sum<G>(qk_total(ss)), inv_d, p.eps));
-      const float pull = qk_sum<G>(qk_total(sg)) * (r * inv_d) * (r * -r);
+      const float r = qk_rsqrt(fmaf(qk_sum<G>(l.live() ? qk_total(ss) : 0.f), inv_d, p.eps));
+      const float pull = qk_sum<G>(l.live() ? qk_total(sg) : 0.f) * (r * inv_d) * (r * -r);
       const f32x2 rr = both(r), pp = both(pull);
 #pragma unroll
-      for (int j = 0; j < NQ; ++j) {
-        f32x2 y1[2], y2[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const f32x2 u = mul2f(g1[j][e], rr), v = mul2f(g2[j][e], rr);
-          if (ok) { dw1[j][e] = fma2f(u, f1[j][e], dw1[j][e]); dw2[j][e] = fma2f(v, f2[j][e], dw2[j][e]); }
-          y1[e] = fma2f(f1[j][e], pp, mul2f(u, w1[j][e]));
-          y2[e] = fma2f(f2[j][e], pp, mul2f(v, w2[j][e]));
-        }
-        if (ok && l.live(j)) {
-          st_quad(dst + l.o1(j), y1);
-          st_quad(dst + l.o2(j), y2);
-        }
+      for (int e = 0; e < 4; ++e) {
+        const f32x2 u = mul2f(g1[e], rr), v = mul2f(g2[e], rr);
+        if (ok) { dw1[e] = fma2f(u, f1[e], dw1[e]); dw2[e] = fma2f(v, f2[e], dw2[e]); }
+        f1[e] = fma2f(f1[e], pp, mul2f(u, w1[e]));
+        f2[e] = fma2f(f2[e], pp, mul2f(v, w2[e]));
       }
-      dst += out_step;
+      if (ok && l.live()) {
+        st_pairs(dst, f1);
+        st_pairs(dst + (l.o2() - l.o1()), f2);
+      }
     }
   }
   if (p.part == nullptr) return;
+  __syncthreads();      // (the ring is empty: nothing is on its way that a warp has not waited for)
+  float* s_part = reinterpret_cast<float*>(s_ring);      // [warp][channel]
 #pragma unroll
-  for (int j = 0; j < NQ; ++j)
+  for (int e = 0; e < 4; ++e) {
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-#pragma unroll
-      for (int o = G; o < 32; o <<= 1) {
-        dw1[j][e] = add2f(dw1[j][e], __shfl_xor_sync(0xffffffffu, (unsigned long long)dw1[j][e], o));
-        dw2[j][e] = add2f(dw2[j][e], __shfl_xor_sync(0xffffffffu, (unsigned long long)dw2[j][e], o));
-      }
-      if (sub == 0 && l.live(j)) {
-        const float2 u = unpair(dw1[j][e]), v = unpair(dw2[j][e]);
-        s_part[warp][l.o1(j) + 2 * e] = u.x; s_part[warp][l.o1(j) + 2 * e + 1] = u.y;
-        s_part[warp][l.o2(j) + 2 * e] = v.x; s_part[warp][l.o2(j) + 2 * e + 1] = v.y;
-      }
+    for (int o = G; o < 32; o <<= 1) {
+      dw1[e] = add2f(dw1[e], __shfl_xor_sync(0xffffffffu, (unsigned long long)dw1[e], o));
+      dw2[e] = add2f(dw2[e], __shfl_xor_sync(0xffffffffu, (unsigned long long)dw2[e], o));
     }
+    if (sub == 0 && l.live()) {
+      const float2 u = unpair(dw1[e]), v = unpair(dw2[e]);
+      float *at1 = s_part + warp * p.d + l.o1() + 2 * e, *at2 = s_part + warp * p.d + l.o2() + 2 * e;
+      at1[0] = u.x; at1[1] = u.y;
+      at2[0] = v.x; at2[1] = v.y;
+    }
+  }
   __syncthreads();
   for (int i = threadIdx.x; i < p.d; i += kQkThreads) {
     float sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < kQkWarps; ++w) sum += s_part[w][i];
+    for (int w = 0; w < kQkWarps; ++w) sum += s_part[w * p.d + i];
     p.part[(int64_t)blockIdx.x * p.d + i] = sum;
   }
 }
@@ -354,10 +368,10 @@ static int qk_check(const hyc_qk_norm* a, bool backward) {
   return HYC_OK;
 }
 
-// lanes of a head: one per eight channels, a power of two; 32 of them with twice as many above 256 channels
+// lanes of a head: one per 16 channels, a power of two
 static int qk_group(int d) {
-  int g = 2;
-  while (g < d / 8 && g < 32) g <<= 1;
+  int g = 1;
+  while (g < d / 16) g <<= 1;
   return g;
 }
 
@@ -399,22 +413,27 @@ static void qk_fill(QkParams& p, const hyc_qk_norm* a) {
   p.part = nullptr;
 }
 
-// f(element, lanes of a head, pairs of quads per lane, FULL)
+// bytes of the ring, and of backward's sums over the warps, which take its place
+template <typename T>
+constexpr int qk_smem(bool backward) { return kQkRing * (backward ? 4 : 2) * kQkThreads * 8 * (int)sizeof(T); }
+static_assert(qk_smem<__half>(true) >= kQkWarps * 512 * 4, "the sums fit in the ring");
+
+// f(element, lanes of a head, FULL)
 template <typename F>
 static int qk_by_type(int type, int d, int rot, F&& f) {
   auto by_group = [&](auto elem) -> int {
     using std::integral_constant;
-    auto full = [&](auto group, auto quads) -> int {
-      if (rot == d && d == 8 * decltype(group)::value * decltype(quads)::value) return f(elem, group, quads, std::true_type());
-      return f(elem, group, quads, std::false_type());
+    auto full = [&](auto group) -> int {
+      if (rot == d && d == 16 * decltype(group)::value) return f(elem, group, std::true_type());
+      return f(elem, group, std::false_type());
     };
-    constexpr integral_constant<int, 1> one{};
     switch (qk_group(d)) {
-      case 2: return full(integral_constant<int, 2>(), one);
-      case 4: return full(integral_constant<int, 4>(), one);
-      case 8: return full(integral_constant<int, 8>(), one);
-      case 16: return full(integral_constant<int, 16>(), one);
-      default: return d <= 256 ? full(integral_constant<int, 32>(), one) : full(integral_constant<int, 32>(), integral_constant<int, 2>());
+      case 1: return full(integral_constant<int, 1>());
+      case 2: return full(integral_constant<int, 2>());
+      case 4: return full(integral_constant<int, 4>());
+      case 8: return full(integral_constant<int, 8>());
+      case 16: return full(integral_constant<int, 16>());
+      default: return full(integral_constant<int, 32>());
     }
   };
   if (type == HYC_F32) return by_group(float());
@@ -431,10 +450,13 @@ extern "C" HYC_API int hyc_qk_norm_rope_fwd(const hyc_qk_norm* a, void* stream) 
   if (rc != HYC_OK || a->batch * a->seq == 0) return rc;
   QkParams p;
   qk_fill(p, a);
-  return qk_by_type(a->type, p.d, 2 * p.half, [&](auto elem, auto group, auto quads, auto full) -> int {
-    auto kern = qk_norm_fwd_kernel<decltype(elem), decltype(group)::value, decltype(quads)::value, decltype(full)::value, 2>;
-    qk_plan(p, num_sms() * resident_blocks(kern, kQkThreads, 0, 2));
-    launch_pdl(kern, dim3((unsigned)(p.t[0].blocks + p.t[1].blocks)), dim3(kQkThreads), 0, (cudaStream_t)stream, p);
+  return qk_by_type(a->type, p.d, 2 * p.half, [&](auto elem, auto group, auto full) -> int {
+    constexpr auto kern = qk_norm_fwd_kernel<decltype(elem), decltype(group)::value, decltype(full)::value>;
+    constexpr int smem = qk_smem<decltype(elem)>(false);
+    const int rs = more_shared_memory<kern>(smem);
+    if (rs != HYC_OK) return rs;
+    qk_plan(p, num_sms() * resident_blocks(kern, kQkThreads, smem, 1));
+    launch_pdl(kern, dim3((unsigned)(p.t[0].blocks + p.t[1].blocks)), dim3(kQkThreads), smem, (cudaStream_t)stream, p);
     HYC_CHECK_LAUNCH();
     return HYC_OK;
   });
@@ -455,11 +477,14 @@ extern "C" HYC_API int hyc_qk_norm_rope_bwd(const hyc_qk_norm* a, void* dweight_
   qk_fill(p, a);
   if (p.tokens > 0) {
     p.part = weights ? (float*)workspace : nullptr;
-    const int r = qk_by_type(a->type, p.d, 2 * p.half, [&](auto elem, auto group, auto quads, auto full) -> int {
-      auto kern = qk_norm_bwd_kernel<decltype(elem), decltype(group)::value, decltype(quads)::value, decltype(full)::value>;
-      const int res = resident_blocks(kern, kQkThreads, 0, 1);
+    const int r = qk_by_type(a->type, p.d, 2 * p.half, [&](auto elem, auto group, auto full) -> int {
+      constexpr auto kern = qk_norm_bwd_kernel<decltype(elem), decltype(group)::value, decltype(full)::value>;
+      constexpr int smem = qk_smem<decltype(elem)>(true);
+      const int rs = more_shared_memory<kern>(smem);
+      if (rs != HYC_OK) return rs;
+      const int res = resident_blocks(kern, kQkThreads, smem, 1);
       qk_plan(p, num_sms() * (res < kQkBwdBlocks ? res : kQkBwdBlocks));
-      launch_pdl(kern, dim3((unsigned)(p.t[0].blocks + p.t[1].blocks)), dim3(kQkThreads), 0, (cudaStream_t)stream, p);
+      launch_pdl(kern, dim3((unsigned)(p.t[0].blocks + p.t[1].blocks)), dim3(kQkThreads), smem, (cudaStream_t)stream, p);
       HYC_CHECK_LAUNCH();
       return HYC_OK;
     });
