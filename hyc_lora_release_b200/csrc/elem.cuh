@@ -98,35 +98,66 @@ __device__ __forceinline__ f32x2 add2f(f32x2 a, f32x2 b) { f32x2 r; asm("add.rn.
 __device__ __forceinline__ f32x2 mul2f(f32x2 a, f32x2 b) { f32x2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
 __device__ __forceinline__ f32x2 fma2f(f32x2 a, f32x2 b, f32x2 c) { f32x2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
 
-// eight adjacent values as four pairs
-__device__ __forceinline__ void octet_to_pairs(const Octet<__nv_bfloat16>& o, f32x2 (&f)[4]) {
-  const uint32_t w[4] = {o.v[0].x, o.v[0].y, o.v[0].z, o.v[0].w};
+// adjacent values as pairs: 16 bytes of 16-bit elements (N = 4), 16 or 32 of fp32 (N = 2, 4)
+__device__ __forceinline__ void bits_to_pairs(const uint4 (&o)[1], f32x2 (&f)[4], __nv_bfloat16) {
+  const uint32_t w[4] = {o[0].x, o[0].y, o[0].z, o[0].w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) f[i] = pair(bf16lo_to_f32(w[i]), bf16hi_to_f32(w[i]));
 }
-__device__ __forceinline__ void octet_to_pairs(const Octet<__half>& o, f32x2 (&f)[4]) {
-  const uint32_t w[4] = {o.v[0].x, o.v[0].y, o.v[0].z, o.v[0].w};
+__device__ __forceinline__ void bits_to_pairs(const uint4 (&o)[1], f32x2 (&f)[4], __half) {
+  const uint32_t w[4] = {o[0].x, o[0].y, o[0].z, o[0].w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) { const float2 t = half2_bits_to_f32(w[i]); f[i] = pair(t.x, t.y); }
 }
-__device__ __forceinline__ void octet_to_pairs(const Octet<float>& o, f32x2 (&f)[4]) {
+template <int P>
+__device__ __forceinline__ void bits_to_pairs(const uint4 (&o)[P], f32x2 (&f)[2 * P], float) {
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    f[2 * i] = pair(__uint_as_float(o.v[i].x), __uint_as_float(o.v[i].y));
-    f[2 * i + 1] = pair(__uint_as_float(o.v[i].z), __uint_as_float(o.v[i].w));
+  for (int i = 0; i < P; ++i) {
+    f[2 * i] = pair(__uint_as_float(o[i].x), __uint_as_float(o[i].y));
+    f[2 * i + 1] = pair(__uint_as_float(o[i].z), __uint_as_float(o[i].w));
   }
 }
-template <typename T>
-__device__ __forceinline__ void st_pairs(T* p, const f32x2 (&f)[4]) {
-  float v[8];
+// one rounding (to nearest even) per value
+__device__ __forceinline__ void st_pairs(__nv_bfloat16* p, const f32x2 (&f)[4]) {
+  uint32_t w[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) { const float2 t = unpair(f[i]); v[2 * i] = t.x; v[2 * i + 1] = t.y; }
-  st_octet(p, v);
+  for (int i = 0; i < 4; ++i) { const float2 t = unpair(f[i]); w[i] = pack_bf16x2_rn(t.x, t.y); }
+  *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
-__device__ __forceinline__ void ld_any_pairs(const void* p, int64_t at, int type, f32x2 (&f)[4]) {
-  if (type == HYC_F32) octet_to_pairs(ld_octet(reinterpret_cast<const float*>(p) + at), f);
-  else if (type == HYC_F16) octet_to_pairs(ld_octet(reinterpret_cast<const __half*>(p) + at), f);
-  else octet_to_pairs(ld_octet(reinterpret_cast<const __nv_bfloat16*>(p) + at), f);
+__device__ __forceinline__ void st_pairs(__half* p, const f32x2 (&f)[4]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { const float2 t = unpair(f[i]); w[i] = f32_to_half2_bits(t.x, t.y); }
+  *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <int N>
+__device__ __forceinline__ void st_pairs(float* p, const f32x2 (&f)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    const float2 a = unpair(f[i]), b = unpair(f[i + 1]);
+    *reinterpret_cast<float4*>(p + 2 * i) = make_float4(a.x, a.y, b.x, b.y);
+  }
+}
+// values of a vector whose type is known at run time, from element `at` on (a multiple of 2 N)
+template <int N>
+__device__ __forceinline__ void ld_any_pairs(const void* p, int64_t at, int type, f32x2 (&f)[N]) {
+  if (type == HYC_F32) {
+    const float4* q = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + at);
+#pragma unroll
+    for (int i = 0; i < N; i += 2) { const float4 v = q[i / 2]; f[i] = pair(v.x, v.y); f[i + 1] = pair(v.z, v.w); }
+    return;
+  }
+  const uint2* q = reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(p) + at);
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    const uint2 v = q[i / 2];
+    if (type == HYC_F16) {
+      const float2 a = half2_bits_to_f32(v.x), b = half2_bits_to_f32(v.y);
+      f[i] = pair(a.x, a.y); f[i + 1] = pair(b.x, b.y);
+    } else {
+      f[i] = pair(bf16lo_to_f32(v.x), bf16hi_to_f32(v.x)); f[i + 1] = pair(bf16lo_to_f32(v.y), bf16hi_to_f32(v.y));
+    }
+  }
 }
 
 inline bool elem_type_ok(int t) { return t == HYC_BF16 || t == HYC_F16 || t == HYC_F32; }

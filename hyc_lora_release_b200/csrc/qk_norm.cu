@@ -28,12 +28,21 @@ __device__ __forceinline__ float qk_rsqrt(float v) {
   return r;
 }
 
+// n / d for n < 2^31 and d >= 1: a multiplication by a rounded-up reciprocal of 33 bits (T. Granlund and P. Montgomery, Division by
+// invariant integers using multiplication)
+struct QkDivisor { uint32_t d, mul, shift; };
+__device__ __forceinline__ uint32_t qk_divide(uint32_t n, const QkDivisor& v) {
+  const uint32_t hi = __umulhi(n, v.mul);
+  return (hi + ((n - hi) >> (v.shift > 0 ? 1 : 0))) >> (v.shift > 0 ? v.shift - 1 : 0);
+}
+
 struct QkTensor {
   const void *x, *dy, *w;
   void* out;                       // contiguous [tokens, heads, d]
   int64_t xb, xm, xh, gb, gm, gh;  // strides of x and dy: batch, token, head
   int heads;
   int splits, per_split;           // a token's head groups as `splits` items of `per_split` groups
+  QkDivisor by_splits;
   int blocks;                      // blocks that work on this tensor
 };
 struct QkParams {
@@ -42,50 +51,50 @@ struct QkParams {
   int64_t ld_cos, ld_sin, pb, pm;  // strides of the positions: batch, token
   int pos64, table_type, w_type, table_rows;
   int tokens, seq, d, half;
+  QkDivisor by_seq;
   float eps;
   float* part;                     // backward: [blocks][d] sums of the weights' gradients, q's blocks first; or null
 };
 
-// The lane's channels of a head: the octets from o1 and from o2 on.  FULL: the head's size is 16 times a power of two and all of it is
-// turned, so that every lane has channels, all of one kind, and partners at a distance known when this is compiled.
-template <int G, bool FULL> struct QkLane {
+// The lane's channels of a head: E adjacent ones from o1 and E from o2 on.  FULL: the head's size is 2 E times a power of two and all of it
+// is turned, so that every lane has channels, all of one kind, and partners at a distance known when this is compiled.
+template <int E, int G, bool FULL> struct QkLane {
   int first, second;
   bool is_live, is_turned;
   __device__ __forceinline__ QkLane(int li, int d, int half) {
-    const int i = li - half / 8;
-    is_live = li < d / 16;
-    is_turned = li < half / 8;
-    first = is_turned ? 8 * li : 2 * half + 16 * i;
-    second = is_turned ? 8 * li + half : 2 * half + 16 * i + 8;
+    const int i = li - half / E;
+    is_live = li < d / (2 * E);
+    is_turned = li < half / E;
+    first = is_turned ? E * li : 2 * half + 2 * E * i;
+    second = is_turned ? E * li + half : 2 * half + 2 * E * i + E;
     if (!is_live) { first = 0; second = 0; }
   }
   __device__ __forceinline__ bool live() const { return FULL || is_live; }
   __device__ __forceinline__ bool turned() const { return FULL || is_turned; }
   __device__ __forceinline__ int o1() const { return first; }
-  __device__ __forceinline__ int o2() const { return FULL ? first + 8 * G : second; }
+  __device__ __forceinline__ int o2() const { return FULL ? first + E * G : second; }
 };
 
 // cos, sin and -sin of a token at the lane's channels; a position outside of the tables gives NaN, and reads nothing
-struct QkAngles { f32x2 c[4], s[4], ns[4]; };
-template <typename L>
-__device__ __forceinline__ void qk_angles(const QkParams& p, int b, int m, const L& l, QkAngles& a) {
+template <int N> struct QkAngles { f32x2 c[N], s[N], ns[N]; };
+template <int N, typename L>
+__device__ __forceinline__ void qk_angles(const QkParams& p, int b, int m, const L& l, QkAngles<N>& a) {
   int64_t at = m;
   if (p.pos != nullptr) {
     const int64_t i = b * p.pb + m * p.pm;
     at = p.pos64 ? reinterpret_cast<const int64_t*>(p.pos)[i] : (int64_t)reinterpret_cast<const int32_t*>(p.pos)[i];
   }
   const bool known = at >= 0 && at < p.table_rows;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    a.c[e] = both(known || !l.turned() ? 1.f : __int_as_float(0x7fc00000));
-    a.s[e] = both(known || !l.turned() ? 0.f : __int_as_float(0x7fc00000));
-  }
   if (l.turned() && known) {
     ld_any_pairs(p.cos_t, at * p.ld_cos + l.o1(), p.table_type, a.c);
     ld_any_pairs(p.sin_t, at * p.ld_sin + l.o1(), p.table_type, a.s);
+  } else {
+    const float nan = __int_as_float(0x7fc00000);
+#pragma unroll
+    for (int e = 0; e < N; ++e) { a.c[e] = both(l.turned() ? nan : 1.f); a.s[e] = both(l.turned() ? nan : 0.f); }
   }
 #pragma unroll
-  for (int e = 0; e < 4; ++e) a.ns[e] = a.s[e] ^ 0x8000000080000000ull;
+  for (int e = 0; e < N; ++e) a.ns[e] = a.s[e] ^ 0x8000000080000000ull;
 }
 
 template <int G>
@@ -102,24 +111,24 @@ __device__ __forceinline__ float qk_total(f32x2 v) {
 struct QkItem { uint32_t token; int first, b, m; };
 __device__ __forceinline__ QkItem qk_item(const QkParams& p, const QkTensor& t, uint32_t item) {
   QkItem i;
-  i.token = item / (uint32_t)t.splits;
+  i.token = qk_divide(item, t.by_splits);
   i.first = (int)(item - i.token * (uint32_t)t.splits) * t.per_split;
-  i.b = (int)(i.token / (uint32_t)p.seq);
+  i.b = (int)qk_divide(i.token, p.by_seq);
   i.m = (int)(i.token - (uint32_t)i.b * (uint32_t)p.seq);
   return i;
 }
 
 // ---- a warp's head groups, those of all its items in a row, on their way into shared memory kQkRing at a time: every lane copies the
-// octets that it will read itself, so that nobody waits for another lane
-constexpr int kQkRing = 4;
+// pieces that it will read itself, so that nobody waits for another lane
+template <typename T> constexpr int kQkRing = sizeof(T) == 4 ? 3 : 4;      // (by shared memory)
 __device__ __forceinline__ void qk_copy(uint32_t to, const void* from) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
-// PER: heads of a warp at a time; BWD: x and dy, else x
-template <typename T, int PER, bool BWD, typename L>
+// E: channels of a piece; PER: heads of a warp at a time; BWD: x and dy, else x
+template <typename T, int E, int PER, bool BWD, typename L>
 struct QkFeed {
-  static constexpr int OCTETS = BWD ? 4 : 2, PARTS = (int)sizeof(T) / 2, STRIDE = kQkThreads * 16;      // 16-byte parts of an octet; of the block's lanes
-  static constexpr int PLACE = OCTETS * PARTS * STRIDE;
+  static constexpr int PIECES = BWD ? 4 : 2, PARTS = E * (int)sizeof(T) / 16, STRIDE = kQkThreads * 16;      // 16-byte parts of a piece; of the block's lanes
+  static constexpr int PLACE = PIECES * PARTS * STRIDE, RING = kQkRing<T>;
   const QkParams& p;
   const QkTensor& t;
   const L& l;
@@ -129,10 +138,10 @@ struct QkFeed {
   int left, sub;
   __device__ __forceinline__ QkFeed(const QkParams& p_, const QkTensor& t_, const L& l_, uint32_t first, uint32_t items_, uint32_t item_step_, int sub_, uint32_t smem)
       : p(p_), t(t_), l(l_), step(PER * t_.xh), grad_step(BWD ? PER * t_.gh : 0), item(first), items(items_), item_step(item_step_),
-        base(smem + threadIdx.x * 16), put(base), got(base), top(base + kQkRing * PLACE), sub(sub_) {
+        base(smem + threadIdx.x * 16), put(base), got(base), top(base + RING * PLACE), sub(sub_) {
     open();
 #pragma unroll
-    for (int i = 0; i < kQkRing - 1; ++i) send();
+    for (int i = 0; i < RING - 1; ++i) send();
   }
   __device__ __forceinline__ void open() {
     if (item >= items) return;
@@ -142,9 +151,9 @@ struct QkFeed {
     src = reinterpret_cast<const T*>(t.x) + it.b * t.xb + it.m * t.xm + head0 * t.xh;
     if (BWD) grad = reinterpret_cast<const T*>(t.dy) + it.b * t.gb + it.m * t.gm + head0 * t.gh;
   }
-  __device__ __forceinline__ void copy(int octet, const T* from) {
+  __device__ __forceinline__ void copy(int piece, const T* from) {
 #pragma unroll
-    for (int i = 0; i < PARTS; ++i) qk_copy(put + (uint32_t)((octet * PARTS + i) * STRIDE), from + i * (16 / (int)sizeof(T)));
+    for (int i = 0; i < PARTS; ++i) qk_copy(put + (uint32_t)((piece * PARTS + i) * STRIDE), from + i * (16 / (int)sizeof(T)));
   }
   // the next group's copies, into the ring's next place (nothing once all are under way: the groups stay countable)
   __device__ __forceinline__ void send() {
@@ -166,14 +175,14 @@ struct QkFeed {
     put += PLACE;
     if (put == top) put = base;
   }
-  __device__ __forceinline__ void wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kQkRing - 2) : "memory"); }
-  __device__ __forceinline__ void take(int octet, f32x2 (&f)[4]) const {
-    Octet<T> o;
+  __device__ __forceinline__ void wait() { asm volatile("cp.async.wait_group %0;" ::"n"(RING - 2) : "memory"); }
+  __device__ __forceinline__ void take(int piece, f32x2 (&f)[E / 2]) const {
+    uint4 o[PARTS];
 #pragma unroll
     for (int i = 0; i < PARTS; ++i)
       asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                   : "=r"(o.v[i].x), "=r"(o.v[i].y), "=r"(o.v[i].z), "=r"(o.v[i].w) : "r"(got + (uint32_t)((octet * PARTS + i) * STRIDE)) : "memory");
-    octet_to_pairs(o, f);
+                   : "=r"(o[i].x), "=r"(o[i].y), "=r"(o[i].z), "=r"(o[i].w) : "r"(got + (uint32_t)((piece * PARTS + i) * STRIDE)) : "memory");
+    bits_to_pairs(o, f, T());
   }
   __device__ __forceinline__ void next() {
     got += PLACE;
@@ -181,7 +190,7 @@ struct QkFeed {
   }
 };
 
-template <typename T, int G, bool FULL>
+template <typename T, int E, int G, bool FULL>
 __global__ void __launch_bounds__(kQkThreads, 3)
 qk_norm_fwd_kernel(const __grid_constant__ QkParams p) {
   extern __shared__ __align__(16) uint8_t s_ring[];
@@ -191,35 +200,36 @@ qk_norm_fwd_kernel(const __grid_constant__ QkParams p) {
   const QkTensor& t = p.t[second ? 1 : 0];
   const int block = (int)blockIdx.x - (second ? p.t[0].blocks : 0);
   const int lane = threadIdx.x & 31, sub = lane / G;
-  typedef QkLane<G, FULL> Lane;
+  typedef QkLane<E, G, FULL> Lane;
+  constexpr int N = E / 2;
   const Lane l(lane % G, p.d, p.half);
   const uint32_t items = (uint32_t)p.tokens * (uint32_t)t.splits, item_step = (uint32_t)t.blocks * kQkWarps;
   const uint32_t first = (uint32_t)block * kQkWarps + (threadIdx.x >> 5);
-  QkFeed<T, PER, false, Lane> feed(p, t, l, first, items, item_step, sub, (uint32_t)__cvta_generic_to_shared(s_ring));
-  f32x2 w1[4], w2[4];
+  QkFeed<T, E, PER, false, Lane> feed(p, t, l, first, items, item_step, sub, (uint32_t)__cvta_generic_to_shared(s_ring));
+  f32x2 w1[N], w2[N];
   ld_any_pairs(t.w, l.o1(), p.w_type, w1);
   ld_any_pairs(t.w, l.o2(), p.w_type, w2);
   const float inv_d = 1.f / (float)p.d;
   const int out_step = PER * p.d;
   for (uint32_t item = first; item < items; item += item_step) {
     const QkItem it = qk_item(p, t, item);
-    QkAngles a;
+    QkAngles<N> a;
     qk_angles(p, it.b, it.m, l, a);
     const int head0 = it.first * PER + sub;
     int left = min((it.first + t.per_split) * PER, t.heads) - head0;
     T* dst = reinterpret_cast<T*>(t.out) + (int64_t)it.token * t.heads * p.d + head0 * p.d + l.o1();
     for (; left > -sub; left -= PER, dst += out_step) {
-      f32x2 f1[4], f2[4], ss = both(0.f);
+      f32x2 f1[N], f2[N], ss = both(0.f);
       feed.wait();
       feed.take(0, f1);
       feed.take(1, f2);
       feed.next();
       feed.send();
 #pragma unroll
-      for (int e = 0; e < 4; ++e) ss = fma2f(f1[e], f1[e], fma2f(f2[e], f2[e], ss));
+      for (int e = 0; e < N; ++e) ss = fma2f(f1[e], f1[e], fma2f(f2[e], f2[e], ss));
       const f32x2 rr = both(qk_rsqrt(fmaf(qk_sum<G>(l.live() ? qk_total(ss) : 0.f), inv_d, p.eps)));
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
+      for (int e = 0; e < N; ++e) {
         const f32x2 n1 = mul2f(mul2f(f1[e], rr), w1[e]), n2 = mul2f(mul2f(f2[e], rr), w2[e]);
         f1[e] = fma2f(n2, a.ns[e], mul2f(n1, a.c[e]));
         f2[e] = fma2f(n1, a.s[e], mul2f(n2, a.c[e]));
@@ -232,7 +242,7 @@ qk_norm_fwd_kernel(const __grid_constant__ QkParams p) {
   }
 }
 
-template <typename T, int G, bool FULL>
+template <typename T, int E, int G, bool FULL>
 __global__ void __launch_bounds__(kQkThreads, kQkBwdBlocks)
 qk_norm_bwd_kernel(const __grid_constant__ QkParams p) {
   extern __shared__ __align__(16) uint8_t s_ring[];
@@ -242,28 +252,29 @@ qk_norm_bwd_kernel(const __grid_constant__ QkParams p) {
   const QkTensor& t = p.t[second ? 1 : 0];
   const int block = (int)blockIdx.x - (second ? p.t[0].blocks : 0);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane / G;
-  typedef QkLane<G, FULL> Lane;
+  typedef QkLane<E, G, FULL> Lane;
+  constexpr int N = E / 2;
   const Lane l(lane % G, p.d, p.half);
   const uint32_t items = (uint32_t)p.tokens * (uint32_t)t.splits, item_step = (uint32_t)t.blocks * kQkWarps;
   const uint32_t first = (uint32_t)block * kQkWarps + (uint32_t)warp;
-  QkFeed<T, PER, true, Lane> feed(p, t, l, first, items, item_step, sub, (uint32_t)__cvta_generic_to_shared(s_ring));
-  f32x2 w1[4], w2[4], dw1[4], dw2[4];
+  QkFeed<T, E, PER, true, Lane> feed(p, t, l, first, items, item_step, sub, (uint32_t)__cvta_generic_to_shared(s_ring));
+  f32x2 w1[N], w2[N], dw1[N], dw2[N];
   ld_any_pairs(t.w, l.o1(), p.w_type, w1);
   ld_any_pairs(t.w, l.o2(), p.w_type, w2);
 #pragma unroll
-  for (int e = 0; e < 4; ++e) dw1[e] = dw2[e] = both(0.f);
+  for (int e = 0; e < N; ++e) dw1[e] = dw2[e] = both(0.f);
   const float inv_d = 1.f / (float)p.d;
   const int out_step = PER * p.d;
   for (uint32_t item = first; item < items; item += item_step) {
     const QkItem it = qk_item(p, t, item);
-    QkAngles a;
+    QkAngles<N> a;
     qk_angles(p, it.b, it.m, l, a);
     const int head0 = it.first * PER + sub;
     int left = min((it.first + t.per_split) * PER, t.heads) - head0;
     T* dst = reinterpret_cast<T*>(t.out) + (int64_t)it.token * t.heads * p.d + head0 * p.d + l.o1();
     for (; left > -sub; left -= PER, dst += out_step) {
       const bool ok = left > 0;
-      f32x2 f1[4], f2[4], g1[4], g2[4], ss = both(0.f), sg = both(0.f);
+      f32x2 f1[N], f2[N], g1[N], g2[N], ss = both(0.f), sg = both(0.f);
       feed.wait();
       feed.take(0, f1);
       feed.take(1, f2);
@@ -272,7 +283,7 @@ qk_norm_bwd_kernel(const __grid_constant__ QkParams p) {
       feed.next();
       feed.send();
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
+      for (int e = 0; e < N; ++e) {
         const f32x2 u = fma2f(g2[e], a.s[e], mul2f(g1[e], a.c[e])), v = fma2f(g1[e], a.ns[e], mul2f(g2[e], a.c[e]));
         ss = fma2f(f1[e], f1[e], fma2f(f2[e], f2[e], ss));
         sg = fma2f(mul2f(u, f1[e]), w1[e], fma2f(mul2f(v, f2[e]), w2[e], sg));
@@ -283,7 +294,7 @@ qk_norm_bwd_kernel(const __grid_constant__ QkParams p) {
       const float pull = qk_sum<G>(l.live() ? qk_total(sg) : 0.f) * (r * inv_d) * (r * -r);
       const f32x2 rr = both(r), pp = both(pull);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
+      for (int e = 0; e < N; ++e) {
         const f32x2 u = mul2f(g1[e], rr), v = mul2f(g2[e], rr);
         if (ok) { dw1[e] = fma2f(u, f1[e], dw1[e]); dw2[e] = fma2f(v, f2[e], dw2[e]); }
         f1[e] = fma2f(f1[e], pp, mul2f(u, w1[e]));
@@ -299,7 +310,7 @@ qk_norm_bwd_kernel(const __grid_constant__ QkParams p) {
   __syncthreads();      // (the ring is empty: nothing is on its way that a warp has not waited for)
   float* s_part = reinterpret_cast<float*>(s_ring);      // [warp][channel]
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
+  for (int e = 0; e < N; ++e) {
 #pragma unroll
     for (int o = G; o < 32; o <<= 1) {
       dw1[e] = add2f(dw1[e], __shfl_xor_sync(0xffffffffu, (unsigned long long)dw1[e], o));
@@ -368,17 +379,24 @@ static int qk_check(const hyc_qk_norm* a, bool backward) {
   return HYC_OK;
 }
 
-// lanes of a head: one per 16 channels, a power of two
-static int qk_group(int d) {
+// Channels of a lane's piece: 16 bytes, so that the lanes of a head read whole lines; fp32 heads of more than 256 channels 32 bytes, for 32 lanes
+static int qk_piece(int type, int d) { return type == HYC_F32 && d <= 256 ? 4 : 8; }
+// lanes of a head, a power of two
+static int qk_group(int type, int d) {
   int g = 1;
-  while (g < d / 16) g <<= 1;
+  while (g < d / (2 * qk_piece(type, d))) g <<= 1;
   return g;
+}
+static QkDivisor qk_divisor(uint32_t d) {
+  uint32_t shift = 0;
+  while ((1ull << shift) < d) ++shift;
+  return {d, (uint32_t)((((1ull << shift) - d) << 32) / d + 1), shift};
 }
 
 // Blocks for the two tensors in proportion to their heads, at most one resident wave and no more than there is work for; a token's head
 // groups are dealt to several warps where that evens out what the warps have to do.
-static void qk_plan(QkParams& p, int wave) {
-  const int per = 32 / qk_group(p.d), heads = p.t[0].heads + p.t[1].heads;
+static void qk_plan(QkParams& p, int group, int wave) {
+  const int per = 32 / group, heads = p.t[0].heads + p.t[1].heads;
   for (int i = 0; i < 2; ++i) {
     QkTensor& t = p.t[i];
     const int groups = (t.heads + per - 1) / per;
@@ -392,6 +410,7 @@ static void qk_plan(QkParams& p, int wave) {
       const int64_t cost = ((int64_t)p.tokens * splits + warps - 1) / warps * (per_split + 2);
       if (best == 0 || cost <= best) { best = cost; t.per_split = per_split; t.splits = splits; }
     }
+    t.by_splits = qk_divisor((uint32_t)t.splits);
     const int64_t need = ((int64_t)p.tokens * t.splits + kQkWarps - 1) / kQkWarps;
     t.blocks = (int)(need < blocks ? need : blocks);
   }
@@ -410,35 +429,40 @@ static void qk_fill(QkParams& p, const hyc_qk_norm* a) {
   p.table_rows = a->table_rows > 0x7fffffffll ? 0x7fffffff : (int)a->table_rows;
   p.tokens = (int)(a->batch * a->seq); p.seq = (int)a->seq; p.d = a->head_dim; p.half = a->rotary_dim / 2;
   p.eps = a->eps;
+  p.by_seq = qk_divisor(p.seq > 0 ? (uint32_t)p.seq : 1u);
   p.part = nullptr;
 }
 
 // bytes of the ring, and of backward's sums over the warps, which take its place
 template <typename T>
-constexpr int qk_smem(bool backward) { return kQkRing * (backward ? 4 : 2) * kQkThreads * 8 * (int)sizeof(T); }
-static_assert(qk_smem<__half>(true) >= kQkWarps * 512 * 4, "the sums fit in the ring");
+constexpr int qk_smem(int piece, bool backward) { return kQkRing<T> * (backward ? 4 : 2) * kQkThreads * piece * (int)sizeof(T); }
+static_assert(qk_smem<__half>(8, true) >= kQkWarps * 512 * 4 && qk_smem<float>(4, true) >= kQkWarps * 256 * 4, "the sums fit in the ring");
 
-// f(element, lanes of a head, FULL)
+// f(element, channels of a piece, lanes of a head, FULL)
 template <typename F>
 static int qk_by_type(int type, int d, int rot, F&& f) {
-  auto by_group = [&](auto elem) -> int {
-    using std::integral_constant;
+  using std::integral_constant;
+  auto by_group = [&](auto elem, auto piece) -> int {
     auto full = [&](auto group) -> int {
-      if (rot == d && d == 16 * decltype(group)::value) return f(elem, group, std::true_type());
-      return f(elem, group, std::false_type());
+      if (rot == d && d == 2 * decltype(piece)::value * decltype(group)::value) return f(elem, piece, group, std::true_type());
+      return f(elem, piece, group, std::false_type());
     };
-    switch (qk_group(d)) {
-      case 1: return full(integral_constant<int, 1>());
-      case 2: return full(integral_constant<int, 2>());
-      case 4: return full(integral_constant<int, 4>());
-      case 8: return full(integral_constant<int, 8>());
-      case 16: return full(integral_constant<int, 16>());
-      default: return full(integral_constant<int, 32>());
+    constexpr bool wide_only = sizeof(elem) == 4 && decltype(piece)::value == 8;      // (fp32 heads of more than 256 channels)
+    if constexpr (!wide_only) {
+      switch (qk_group(type, d)) {
+        case 1: return full(integral_constant<int, 1>());
+        case 2: return full(integral_constant<int, 2>());
+        case 4: return full(integral_constant<int, 4>());
+        case 8: return full(integral_constant<int, 8>());
+        case 16: return full(integral_constant<int, 16>());
+        default: break;
+      }
     }
+    return full(integral_constant<int, 32>());
   };
-  if (type == HYC_F32) return by_group(float());
-  if (type == HYC_F16) return by_group(__half());
-  return by_group(__nv_bfloat16());
+  if (type == HYC_F32) return qk_piece(type, d) == 4 ? by_group(float(), integral_constant<int, 4>()) : by_group(float(), integral_constant<int, 8>());
+  if (type == HYC_F16) return by_group(__half(), integral_constant<int, 8>());
+  return by_group(__nv_bfloat16(), integral_constant<int, 8>());
 }
 
 }  // namespace hyc
@@ -450,12 +474,12 @@ extern "C" HYC_API int hyc_qk_norm_rope_fwd(const hyc_qk_norm* a, void* stream) 
   if (rc != HYC_OK || a->batch * a->seq == 0) return rc;
   QkParams p;
   qk_fill(p, a);
-  return qk_by_type(a->type, p.d, 2 * p.half, [&](auto elem, auto group, auto full) -> int {
-    constexpr auto kern = qk_norm_fwd_kernel<decltype(elem), decltype(group)::value, decltype(full)::value>;
-    constexpr int smem = qk_smem<decltype(elem)>(false);
+  return qk_by_type(a->type, p.d, 2 * p.half, [&](auto elem, auto piece, auto group, auto full) -> int {
+    constexpr auto kern = qk_norm_fwd_kernel<decltype(elem), decltype(piece)::value, decltype(group)::value, decltype(full)::value>;
+    constexpr int smem = qk_smem<decltype(elem)>(decltype(piece)::value, false);
     const int rs = more_shared_memory<kern>(smem);
     if (rs != HYC_OK) return rs;
-    qk_plan(p, num_sms() * resident_blocks(kern, kQkThreads, smem, 1));
+    qk_plan(p, decltype(group)::value, num_sms() * resident_blocks(kern, kQkThreads, smem, 1));
     launch_pdl(kern, dim3((unsigned)(p.t[0].blocks + p.t[1].blocks)), dim3(kQkThreads), smem, (cudaStream_t)stream, p);
     HYC_CHECK_LAUNCH();
     return HYC_OK;
@@ -477,13 +501,13 @@ extern "C" HYC_API int hyc_qk_norm_rope_bwd(const hyc_qk_norm* a, void* dweight_
   qk_fill(p, a);
   if (p.tokens > 0) {
     p.part = weights ? (float*)workspace : nullptr;
-    const int r = qk_by_type(a->type, p.d, 2 * p.half, [&](auto elem, auto group, auto full) -> int {
-      constexpr auto kern = qk_norm_bwd_kernel<decltype(elem), decltype(group)::value, decltype(full)::value>;
-      constexpr int smem = qk_smem<decltype(elem)>(true);
+    const int r = qk_by_type(a->type, p.d, 2 * p.half, [&](auto elem, auto piece, auto group, auto full) -> int {
+      constexpr auto kern = qk_norm_bwd_kernel<decltype(elem), decltype(piece)::value, decltype(group)::value, decltype(full)::value>;
+      constexpr int smem = qk_smem<decltype(elem)>(decltype(piece)::value, true);
       const int rs = more_shared_memory<kern>(smem);
       if (rs != HYC_OK) return rs;
       const int res = resident_blocks(kern, kQkThreads, smem, 1);
-      qk_plan(p, num_sms() * (res < kQkBwdBlocks ? res : kQkBwdBlocks));
+      qk_plan(p, decltype(group)::value, num_sms() * (res < kQkBwdBlocks ? res : kQkBwdBlocks));
       launch_pdl(kern, dim3((unsigned)(p.t[0].blocks + p.t[1].blocks)), dim3(kQkThreads), smem, (cudaStream_t)stream, p);
       HYC_CHECK_LAUNCH();
       return HYC_OK;
