@@ -566,8 +566,8 @@ linear_slices_kernel(const __grid_constant__ CUtensorMap map_c, const __grid_con
 constexpr int D_ROWS = 8, D_COLS = 256;
 template <typename T>
 __global__ void __launch_bounds__(256)
-linear_dpre_kernel(const T* __restrict__ dy, int64_t ld_dy, const T* __restrict__ pre, T* __restrict__ dpre, float* __restrict__ part, int rows, int n, int per,
-                   int act) {
+linear_dpre_kernel(const T* __restrict__ dy, int64_t ld_dy, const T* __restrict__ pre, T* __restrict__ dpre, float* __restrict__ part, T* __restrict__ dbias,
+                   int rows, int n, int per, int act) {
   __shared__ float s_sum[D_ROWS][D_COLS];
   pdl_wait();
   const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5;
@@ -594,7 +594,7 @@ linear_dpre_kernel(const T* __restrict__ dy, int64_t ld_dy, const T* __restrict_
       }
     });
   }
-  if (part == nullptr) return;
+  if (part == nullptr && dbias == nullptr) return;
 #pragma unroll
   for (int e = 0; e < 8; ++e) s_sum[rl][8 * cl + e] = sum[e];
   __syncthreads();
@@ -602,7 +602,10 @@ linear_dpre_kernel(const T* __restrict__ dy, int64_t ld_dy, const T* __restrict_
 #pragma unroll
   for (int r = 0; r < D_ROWS; ++r) total += s_sum[r][threadIdx.x];
   const int at = (int)blockIdx.x * D_COLS + (int)threadIdx.x;
-  if (at < n) part[(int64_t)blockIdx.y * n + at] = total;
+  if (at < n) {
+    if (dbias != nullptr) dbias[at] = from_f32<T>(total);      // (all rows are this block's)
+    else part[(int64_t)blockIdx.y * n + at] = total;
+  }
 }
 template <typename T>
 __global__ void __launch_bounds__(1024)
@@ -669,7 +672,8 @@ static TilePlan plan_tiles(const Shape& s) {
   const int tiles_m = (s.R + 2 * BM - 1) / (2 * BM), halves = (s.C + BN / 2 - 1) / (BN / 2), pairs = num_sms() / 2;
   const float block = 547.f * (float)((s.K + BK - 1) / BK), half = 0.71f;
   TilePlan best = {0, halves, 1e30f};
-  for (int w = halves / 2; w >= 0; --w) {
+  const int fewest = (int64_t)tiles_m * (halves / 2) > 16ll * pairs ? halves / 2 : 0;      // (of many rounds the last one does not matter)
+  for (int w = halves / 2; w >= fewest; --w) {
     const int64_t wide = (int64_t)tiles_m * w, narrow = (int64_t)tiles_m * (halves - 2 * w);
     const int64_t rounds = wide / pairs, rest = wide % pairs, behind = narrow - (pairs - rest);      // wide tiles are dealt first
     float rest_cost = rounds + half * (float)((narrow + pairs - 1) / pairs);
@@ -769,6 +773,7 @@ static int dpre_rows(int64_t rows, int n) {
   int64_t parts = ((int64_t)num_sms() * 6 + blocks - 1) / blocks;      // about six blocks of 256 threads per SM
   parts = parts > kDpreParts ? kDpreParts : parts < 1 ? 1 : parts;
   int64_t per = (rows + parts - 1) / parts;
+  if (rows <= 64) per = 64;      // eight rows per thread take less than the launch that adds up blocks
   return (int)((per + D_ROWS - 1) / D_ROWS * D_ROWS);
 }
 
@@ -779,10 +784,10 @@ static int launch_dpre(const void* dy, int64_t ld_dy, const void* pre, void* dpr
     const int per = dpre_rows(rows, n);
     parts = (int)((rows + per - 1) / per);
     launch_pdl(linear_dpre_kernel<T>, dim3((unsigned)((n + D_COLS - 1) / D_COLS), (unsigned)parts), dim3(256), 0, st, (const T*)dy, ld_dy, (const T*)pre, (T*)dpre,
-               dbias != nullptr ? part : nullptr, (int)rows, n, per, act);
+               dbias != nullptr && parts > 1 ? part : nullptr, dbias != nullptr && parts == 1 ? (T*)dbias : (T*)nullptr, (int)rows, n, per, act);
     HYC_CHECK_LAUNCH();
   }
-  if (dbias != nullptr) {
+  if (dbias != nullptr && parts != 1) {
     launch_pdl(linear_dbias_kernel<T>, dim3((unsigned)((n + 31) / 32)), dim3(1024), 0, st, (const float*)part, parts, n, (T*)dbias);
     HYC_CHECK_LAUNCH();
   }

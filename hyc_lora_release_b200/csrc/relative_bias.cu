@@ -367,10 +367,10 @@ __device__ __forceinline__ void rb_range(const RbParams& p, const int* edges, in
   if (p.both && k >= p.side) {
     k -= p.side;
     from = max(1, edges[k]);
-    to = k + 1 < p.side ? edges[k + 1] - 1 : 0x3fffffff;
+    to = k + 1 < p.side ? edges[k + 1] - 1 : 0x7ffffff0;
   } else {
-    to = k == 0 && !p.both ? 0x3fffffff : -edges[k];
-    from = k + 1 < p.side ? 1 - edges[k + 1] : -0x3fffffff;
+    to = k == 0 && !p.both ? 0x7ffffff0 : -edges[k];
+    from = k + 1 < p.side ? 1 - edges[k + 1] : -0x7ffffff0;
   }
 }
 
@@ -605,13 +605,13 @@ static void rb_fill(RbParams& p, const hyc_relative_bias* a, const RbPlan& r) {
   for (int i = 0; i < a->side; ++i) p.edges[i] = a->host_edges[i];
 }
 
-template <typename K>
-static int rb_launch(K kern, const RbPlan& r, int64_t blocks, size_t smem, const RbParams& p, cudaStream_t st) {
+// the most dynamic shared memory of any plan: forward a mask and the bias of 16384 columns, backward the diagonals of 16 warps
+constexpr int kRbSmemFwd = (16384 + (16384 + 32 * kRbNarrowWarps) * 9 / 8 + 2) * 4, kRbSmemBwd = kRbMaxWarps * (1024 + 32) * 4;
+template <auto KERN>
+static int rb_launch(int most, const RbPlan& r, int64_t blocks, size_t smem, const RbParams& p, cudaStream_t st) {
   if (blocks > 0x7fffffffll) return HYC_ERR_SHAPE;
-  if (smem > 32768 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
-    hyc_set_last_cuda_error((int)cudaGetLastError());
-    return HYC_ERR_LAUNCH;
-  }
+  const int rc = more_shared_memory<KERN>(most);
+  if (rc != HYC_OK) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)blocks);
   cfg.blockDim = dim3((unsigned)(32 * r.warps));
@@ -624,7 +624,7 @@ static int rb_launch(K kern, const RbPlan& r, int64_t blocks, size_t smem, const
   at[1].val.clusterDim.x = (unsigned)r.cluster; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = r.cluster > 1 ? 2 : 1;
-  if (cudaLaunchKernelEx(&cfg, kern, p) != cudaSuccess) {
+  if (cudaLaunchKernelEx(&cfg, KERN, p) != cudaSuccess) {
     hyc_set_last_cuda_error((int)cudaGetLastError());
     return HYC_ERR_LAUNCH;
   }
@@ -683,16 +683,16 @@ extern "C" HYC_API int hyc_softmax_relative_bias_fwd(const hyc_relative_bias* a,
   const int width = 32 * r.v * r.nv * (r.wide ? r.warps : 1);      // columns of a block
   p.mask_staged = a->mask != nullptr && (a->mask_row == 0 || a->n == 1) ? width : 0;
   return rb_by_plan(a->type, r, [&](auto elem, auto v, auto nv, auto wide) -> int {
-    auto kern = relbias_fwd_kernel<decltype(elem), decltype(v)::value, decltype(nv)::value, decltype(wide)::value>;
+    constexpr auto kern = relbias_fwd_kernel<decltype(elem), decltype(v)::value, decltype(nv)::value, decltype(wide)::value>;
     auto bytes = [&](int rows) { return (size_t)(p.mask_staged + (width + rows) * 9 / 8 + 2) * sizeof(float); };
     const int block_warps = r.wide ? 1 : kRbNarrowWarps;      // warps with rows of their own
-    const int resident = bytes(32 * block_warps) > 32768 ? 1 : resident_blocks(kern, 32 * r.warps, bytes(32 * block_warps), 1);
+    const int resident = resident_blocks(kern, 32 * r.warps, bytes(32 * block_warps), 1);
     const int64_t slots = (int64_t)num_sms() * resident / r.cluster;
     p.rows_per = rb_rows_per(a->batch * a->heads, (int)a->n, block_warps, slots < 1 ? 1 : slots, 3.f, a->causal != 0);
     const int rows = p.rows_per * block_warps;      // of a block
     p.chunks = (int)((a->n + rows - 1) / rows);
     const size_t smem = bytes(rows);
-    return rb_launch(kern, r, a->batch * a->heads * p.chunks * r.cluster, smem, p, (cudaStream_t)stream);
+    return rb_launch<kern>(kRbSmemFwd, r, a->batch * a->heads * p.chunks * r.cluster, smem, p, (cudaStream_t)stream);
   });
 }
 
@@ -720,8 +720,8 @@ extern "C" HYC_API int hyc_softmax_relative_bias_bwd(const hyc_relative_bias* a,
     const int64_t blocks = r.wide ? u.units * r.cluster : (u.units + kRbBwdWarps - 1) / kRbBwdWarps;
     const size_t smem = (size_t)r.warps * (size_t)(32 * r.v * r.nv + u.rows_per) * sizeof(float);
     const int rl = rb_by_plan(a->type, r, [&](auto elem, auto v, auto nv, auto wide) -> int {
-      return rb_launch(relbias_bwd_kernel<decltype(elem), decltype(v)::value, decltype(nv)::value, decltype(wide)::value>, r, blocks, smem, p,
-                       (cudaStream_t)stream);
+      constexpr auto kern = relbias_bwd_kernel<decltype(elem), decltype(v)::value, decltype(nv)::value, decltype(wide)::value>;
+      return rb_launch<kern>(kRbSmemBwd, r, blocks, smem, p, (cudaStream_t)stream);
     });
     if (rl != HYC_OK) return rl;
   }
