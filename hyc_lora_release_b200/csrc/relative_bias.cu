@@ -362,6 +362,44 @@ relbias_fwd_kernel(const __grid_constant__ RbParams p) {
   }
 }
 
+// Backward's rows to come.  Short ones wait in registers; from 32 elements per lane on they would take a quarter of all registers, so they
+// travel into shared memory (cp.async), where every lane reads only what it copied itself, and more warps fit on an SM ([1,32,2048,2048]
+// 162 -> 135 us, causal 120 -> 103).  Not fp32, whose octets are two copies that share their sectors (1000 columns 117 -> 206 us), and not
+// rows that several warps share, whose registers are few enough.
+template <typename T, int V, int NV, bool WIDE>
+struct RbRow {
+  static constexpr bool STAGED = V == 8 && NV >= 4 && sizeof(T) == 2 && !WIDE;
+  static constexpr int BYTES = STAGED ? 2 * NV * 512 : 0;               // of a warp, both operands
+  Piece<T, V> reg[STAGED ? 1 : 2 * NV];
+  uint32_t at;
+  __device__ __forceinline__ explicit RbRow(uint32_t warp_base) : at(warp_base + (threadIdx.x & 31) * 16) {}
+  // slot: 2 k for the probabilities, 2 k + 1 for their gradient, of piece k
+  __device__ __forceinline__ void fetch(int slot, const T* from) {
+    if constexpr (STAGED) {
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + (uint32_t)(slot * 512)), "l"(from) : "memory");
+    } else {
+      ld_piece(from, reg[slot]);
+    }
+  }
+  __device__ __forceinline__ void wait() {
+    if constexpr (STAGED) asm volatile("cp.async.wait_all;" ::: "memory");
+  }
+  __device__ __forceinline__ void get(int slot, float (&f)[V]) const {
+    if constexpr (STAGED) {
+      Octet<T> o;
+      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(o.v[0].x), "=r"(o.v[0].y), "=r"(o.v[0].z), "=r"(o.v[0].w) : "r"(at + (uint32_t)(slot * 512)) : "memory");
+      octet_to_f32(o, f);
+    } else {
+      piece_f32(reg[slot], f);
+    }
+  }
+};
+// floats of shared memory per warp: the row to come, and after the last row the diagonals' sums in its place; sums that left the warp's columns
+__host__ __device__ constexpr int rb_warp_floats(int span, int rows, int staged_bytes) {
+  return ((staged_bytes / 4 > span ? staged_bytes / 4 : span) + rows + 3) / 4 * 4;
+}
+
 // the distances of bucket k: from .. to
 __device__ __forceinline__ void rb_range(const RbParams& p, const int* edges, int k, int& from, int& to) {
   if (p.both && k >= p.side) {
@@ -374,13 +412,12 @@ __device__ __forceinline__ void rb_range(const RbParams& p, const int* edges, in
   }
 }
 
-// Blocks per SM that the registers of a narrow kernel are cut for: 3 (168 registers) where a lane has 64 elements, or 32 that take a
-// register each
-template <typename T, int V, int NV> constexpr int kRbBwdBlocks = V * NV == 64 || (V * NV == 32 && (V == 1 || sizeof(T) == 4)) ? 3 : 4;
+// blocks per SM that the registers of a narrow kernel are cut for
+__host__ __device__ constexpr int rb_bwd_blocks(int bytes, int v, int nv) { return v * nv < 32 ? 4 : bytes == 4 || v == 1 ? 3 : v == 8 && nv == 4 ? 5 : 4; }
 template <typename T, int V, int NV, bool WIDE>
-__global__ void __launch_bounds__(WIDE ? 32 * kRbMaxWarps : 32 * kRbBwdWarps, WIDE ? 1 : kRbBwdBlocks<T, V, NV>)
+__global__ void __launch_bounds__(WIDE ? 32 * kRbMaxWarps : 32 * kRbBwdWarps, WIDE ? 1 : rb_bwd_blocks(sizeof(T), V, NV))
 relbias_bwd_kernel(const __grid_constant__ RbParams p) {
-  extern __shared__ float s_diag_all[];
+  extern __shared__ __align__(16) float s_diag_all[];
   __shared__ int s_edges[kRbMaxSide];
   __shared__ RbExchange s_ex;
   constexpr int SPAN = 32 * V * NV;
@@ -395,18 +432,20 @@ relbias_bwd_kernel(const __grid_constant__ RbParams p) {
   if (!WIDE && unit >= p.units) return;
   const int bh = (int)(unit / p.chunks), chunk = p.chunks - 1 - (int)(unit - (int64_t)bh * p.chunks);      // (causal: long rows first)
   const int first = chunk * p.rows_per, last = min(first + p.rows_per, p.n) - 1;
-  float* s_diag = s_diag_all + warp * (SPAN + p.rows_per);
+  typedef RbRow<T, V, NV, WIDE> Row;
+  float* s_diag = s_diag_all + warp * rb_warp_floats(SPAN, p.rows_per, Row::BYTES);
+  float* s_flush = s_diag + (Row::STAGED ? max(SPAN, Row::BYTES / 4) : SPAN);
   const int c0 = WIDE ? (rank * warps + warp) * SPAN : 0;
   const int64_t map = (int64_t)bh * p.n;
   const int cl = c0 + lane * V;
   const T *a = reinterpret_cast<const T*>(p.x) + (map + first) * p.cols + cl, *g = reinterpret_cast<const T*>(p.grad) + (map + first) * p.cols + cl;
   T* dst = reinterpret_cast<T*>(p.out) + (map + first) * p.cols + cl;
-  Piece<T, V> ra[NV], rg[NV];           // the row to come
+  Row next((uint32_t)__cvta_generic_to_shared(s_diag));
   {
     const int end = rb_end(p, first);
 #pragma unroll
     for (int k = 0; k < NV; ++k)
-      if (cl + k * 32 * V < end) { ld_piece(a + k * 32 * V, ra[k]); ld_piece(g + k * 32 * V, rg[k]); }
+      if (cl + k * 32 * V < end) { next.fetch(2 * k, a + k * 32 * V); next.fetch(2 * k + 1, g + k * 32 * V); }
   }
   float acc[NV][V];
 #pragma unroll
@@ -417,6 +456,7 @@ relbias_bwd_kernel(const __grid_constant__ RbParams p) {
   for (int i = first; i <= last; ++i, turn ^= 1, dst += p.cols) {
     const int end = rb_end(p, i);
     const int end_next = i < last ? rb_end(p, i + 1) : 0;
+    next.wait();
     a += p.cols;
     g += p.cols;
     float dots[V], dot = 0.f;
@@ -427,8 +467,8 @@ relbias_bwd_kernel(const __grid_constant__ RbParams p) {
       const int cb = c0 + k * 32 * V, c = cb + lane * V;
       if (cb >= end) continue;           // (the whole warp, as below)
       float fa[V], fg[V];
-      piece_f32(ra[k], fa);
-      piece_f32(rg[k], fg);
+      next.get(2 * k, fa);
+      next.get(2 * k + 1, fg);
       if (cb + 32 * V <= end) {
         mul_all(fa, fg);
         add_all(dots, fa);
@@ -448,9 +488,9 @@ relbias_bwd_kernel(const __grid_constant__ RbParams p) {
     for (int k = 0; k < NV; ++k) {
       const int cb = c0 + k * 32 * V, c = cb + lane * V;
       float ds[V], o[V], fg[V];
-      piece_f32(ra[k], ds);
-      piece_f32(rg[k], fg);
-      if (c < end_next) { ld_piece(a + k * 32 * V, ra[k]); ld_piece(g + k * 32 * V, rg[k]); }      // (the places are free: the next row's are on their way)
+      next.get(2 * k, ds);
+      next.get(2 * k + 1, fg);
+      if (c < end_next) { next.fetch(2 * k, a + k * 32 * V); next.fetch(2 * k + 1, g + k * 32 * V); }      // (the places are free: the next row's are on their way)
       if (cb >= end) {
 #pragma unroll
         for (int e = 0; e < V; ++e) { ds[e] = 0.f; o[e] = 0.f; }
@@ -475,14 +515,16 @@ relbias_bwd_kernel(const __grid_constant__ RbParams p) {
       for (int e = V - 1; e > 0; --e) acc[k][e] = acc[k][e - 1] + ds[e];
       acc[k][0] = carry + ds[0];
     }
-    if (lane == 0 && i > first) s_diag[SPAN + last - i] = left;
+    if (lane == 0 && i > first) s_flush[last - i] = left;
   }
+  __syncwarp();
 #pragma unroll
   for (int k = 0; k < NV; ++k)
 #pragma unroll
     for (int e = 0; e < V; ++e) s_diag[k * 32 * V + lane * V + e] = acc[k][e];
   __syncwarp();
-  // s_diag[x] is the sum of the diagonal at distance x + dmin
+  // the sum of the diagonal at distance dmin + x: s_diag[x], behind the warp's columns s_flush[x - SPAN]
+  auto diagonal = [&](int x) { return x < SPAN ? s_diag[x] : s_flush[x - SPAN]; };
   const int dmin = c0 - last - p.q_offset, dmax = dmin + SPAN - 1 + (last - first);
   float* part = p.part + ((WIDE ? unit * p.cluster * warps + rank * warps + warp : unit)) * p.buckets;
   // short ranges by a lane each, long ones by the warp
@@ -494,11 +536,11 @@ relbias_bwd_kernel(const __grid_constant__ RbParams p) {
     const bool wide_range = to - from >= 48;
     float sum = 0.f;
     if (!wide_range)
-      for (int d = from; d <= to; ++d) sum += s_diag[d - dmin];
+      for (int d = from; d <= to; ++d) sum += diagonal(d - dmin);
     for (unsigned left = __ballot_sync(0xffffffffu, wide_range); left != 0u; left &= left - 1u) {
       const int l = __ffs(left) - 1, lo = __shfl_sync(0xffffffffu, from, l), hi = __shfl_sync(0xffffffffu, to, l);
       float v = 0.f;
-      for (int d = lo + lane; d <= hi; d += 32) v += s_diag[d - dmin];
+      for (int d = lo + lane; d <= hi; d += 32) v += diagonal(d - dmin);
       v = warp_sum(v);
       if (lane == l) sum = v;
     }
@@ -661,7 +703,7 @@ static int rb_by_plan(int type, const RbPlan& r, F&& f) {
 struct RbUnits { int rows_per, chunks; int64_t units, sums; };
 static RbUnits rb_units(const hyc_relative_bias* a, const RbPlan& r) {
   RbUnits u;
-  const int64_t warps = r.v * r.nv == 64 || (r.v * r.nv == 32 && (r.v == 1 || a->type == HYC_F32)) ? 12 : 16;      // resident per SM: kRbBwdBlocks
+  const int64_t warps = r.wide ? 16 : kRbBwdWarps * rb_bwd_blocks(elem_bytes(a->type), r.v, r.nv);      // resident per SM
   const int64_t slots = (int64_t)num_sms() * warps / (r.wide ? r.warps * r.cluster : 1);
   u.rows_per = rb_rows_per(a->batch * a->heads, (int)a->n, 1, slots < 1 ? 1 : slots, 6.f, a->causal != 0);
   u.chunks = (int)((a->n + u.rows_per - 1) / u.rows_per);
@@ -718,9 +760,10 @@ extern "C" HYC_API int hyc_softmax_relative_bias_bwd(const hyc_relative_bias* a,
     p.part = (float*)workspace;
     p.rows_per = u.rows_per; p.chunks = u.chunks; p.units = u.units;
     const int64_t blocks = r.wide ? u.units * r.cluster : (u.units + kRbBwdWarps - 1) / kRbBwdWarps;
-    const size_t smem = (size_t)r.warps * (size_t)(32 * r.v * r.nv + u.rows_per) * sizeof(float);
     const int rl = rb_by_plan(a->type, r, [&](auto elem, auto v, auto nv, auto wide) -> int {
       constexpr auto kern = relbias_bwd_kernel<decltype(elem), decltype(v)::value, decltype(nv)::value, decltype(wide)::value>;
+      constexpr int V = decltype(v)::value, NV = decltype(nv)::value;
+      const size_t smem = (size_t)r.warps * (size_t)rb_warp_floats(32 * V * NV, u.rows_per, RbRow<decltype(elem), V, NV, decltype(wide)::value>::BYTES) * sizeof(float);
       return rb_launch<kern>(kRbSmemBwd, r, blocks, smem, p, (cudaStream_t)stream);
     });
     if (rl != HYC_OK) return rl;
