@@ -85,11 +85,10 @@ __device__ __forceinline__ float exp2_neg(float v) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
-// a mask's value times log2(e): a finite one stays finite (the type's lowest value must not become -infinity)
-constexpr float kLowest = -3.402823466e38f;
+// a mask's value times log2(e); where that is beyond fp32 as it is: the type's lowest value must not become -infinity
 __device__ __forceinline__ float mask_log2e(float m) {
   const float v = m * kLog2e;
-  return v == -INFINITY && m != -INFINITY ? kLowest : v;
+  return v < -3.402823466e38f ? m : v;
 }
 
 // ---- two fp32 operations per instruction, over the V values of a piece
@@ -267,7 +266,7 @@ relbias_fwd_kernel(const __grid_constant__ RbParams p) {
     const int shift = q_last - q, within = V == 8 ? shift & 7 : 0;
     const float* lut = V == 8 ? s_lut + 9 * ((cl - block_c0) / 8 + (shift >> 3)) : s_lut + (cl - block_c0 + shift);
     src += p.cols;
-    float f[NV][V], m = -INFINITY;
+    float f[NV][V], m, tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};      // (four chains)
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int cb = c0 + k * 32 * V, c = cb + lane * V;
@@ -323,9 +322,9 @@ relbias_fwd_kernel(const __grid_constant__ RbParams p) {
         for (int e = 0; e < V; ++e) f[k][e] = c + e < end ? f[k][e] : -INFINITY;
       }
 #pragma unroll
-      for (int e = 0; e < V; ++e) m = fmaxf(m, f[k][e]);
+      for (int e = 0; e < V; ++e) tops[(k * V + e) & 3] = fmaxf(tops[(k * V + e) & 3], f[k][e]);
     }
-    m = warp_max(m);
+    m = warp_max(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])));
     const float mm = m == -INFINITY ? 0.f : m;      // nothing counts: 2^-inf = 0 everywhere
     float sums[V], sum = 0.f;
 #pragma unroll
