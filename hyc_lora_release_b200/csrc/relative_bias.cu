@@ -266,13 +266,16 @@ relbias_fwd_kernel(const __grid_constant__ RbParams p) {
     const int shift = q_last - q, within = V == 8 ? shift & 7 : 0;
     const float* lut = V == 8 ? s_lut + 9 * ((cl - block_c0) / 8 + (shift >> 3)) : s_lut + (cl - block_c0 + shift);
     src += p.cols;
-    float f[NV][V], m, tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};      // (four chains)
+    // The first NA pieces of the row, in one straight line.  A causal row that ends in its first half leaves the other half out; a branch
+    // per piece would cost more than it saves ([1,32,2048,2048] 87 -> 96 us).
+    auto row = [&](auto pieces) {
+      constexpr int NA = decltype(pieces)::value;
+    float f[NA][V], m, tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};      // (four chains)
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
+    for (int k = 0; k < NA; ++k) {
       const int cb = c0 + k * 32 * V, c = cb + lane * V;
       piece_f32(raw[k], f[k]);
       if (c < end_next) ld_piece(src + k * 32 * V, raw[k]);      // (its place is free: the next row's is on its way from here on)
-      if (cb >= end) continue;           // (the whole warp)
       float bias[V];
 #pragma unroll
       for (int e = 0; e < V; ++e) bias[e] = V == 8 ? lut[k * 32 * 9 + lut_at<V>(within + e)] : lut[k * 32 * V + e];
@@ -280,7 +283,7 @@ relbias_fwd_kernel(const __grid_constant__ RbParams p) {
     }
     if (p.mask_staged) {
 #pragma unroll
-      for (int k = 0; k < NV; ++k) {
+      for (int k = 0; k < NA; ++k) {
         // (behind the row's last column: whatever lies there, the columns do not count)
         float mk[V];
         if constexpr (V == 8) {
@@ -295,7 +298,7 @@ relbias_fwd_kernel(const __grid_constant__ RbParams p) {
     } else if (p.mask != nullptr) {
       const int64_t at = b * p.mask_b + h * p.mask_h + (int64_t)i * p.mask_row + cl;
 #pragma unroll
-      for (int k = 0; k < NV; ++k) {
+      for (int k = 0; k < NA; ++k) {
         if (cl + k * 32 * V >= end) continue;
         float mk[V];
         if constexpr (V == 8) {
@@ -315,7 +318,7 @@ relbias_fwd_kernel(const __grid_constant__ RbParams p) {
       }
     }
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
+    for (int k = 0; k < NA; ++k) {
       const int cb = c0 + k * 32 * V, c = cb + lane * V;
       if (cb + 32 * V > end) {           // (else all of the warp's columns count)
 #pragma unroll
@@ -330,8 +333,7 @@ relbias_fwd_kernel(const __grid_constant__ RbParams p) {
 #pragma unroll
     for (int e = 0; e < V; ++e) sums[e] = 0.f;
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      if (c0 + k * 32 * V >= end) continue;
+    for (int k = 0; k < NA; ++k) {
       add_one(f[k], -mm);
 #pragma unroll
       for (int e = 0; e < V; ++e) f[k][e] = exp2_neg(f[k][e]);
@@ -349,7 +351,7 @@ relbias_fwd_kernel(const __grid_constant__ RbParams p) {
       factor = sum == 0.f ? 0.f : __fdividef(1.f, sum);        // a row that nothing is visible to: zeros
     }
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
+    for (int k = 0; k < NA; ++k) {
       const int cb = c0 + k * 32 * V, c = cb + lane * V;
       mul_one(f[k], factor);
       if (cb + 32 * V > end) {
@@ -358,6 +360,21 @@ relbias_fwd_kernel(const __grid_constant__ RbParams p) {
       }
       if (c < p.cols) st_piece(dst + k * 32 * V, f[k]);
     }
+#pragma unroll
+    for (int k = NA; k < NV; ++k) {      // columns behind the row's end
+      const int c = cl + k * 32 * V;
+      if (c < end_next) ld_piece(src + k * 32 * V, raw[k]);
+      if (c < p.cols) {
+        float zero[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) zero[e] = 0.f;
+        st_piece(dst + k * 32 * V, zero);
+      }
+    }
+    };
+    // (not where warps meet: all of them have to be on the same line)
+    if (!WIDE && NV >= 4 && end <= SPAN / 2) row(std::integral_constant<int, NV >= 4 ? NV / 2 : NV>());
+    else row(std::integral_constant<int, NV>());
   }
 }
 
