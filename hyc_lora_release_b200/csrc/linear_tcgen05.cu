@@ -563,9 +563,9 @@ linear_slices_kernel(const __grid_constant__ CUtensorMap map_c, const __grid_con
 // ------------------------------------------------------------------ dpre and the bias gradient
 // dpre = dy act'(pre) and the column sums of dpre, in one pass.  A thread has eight columns (128-bit accesses) of every eighth row of the
 // block's rows; sums per thread, per block in a fixed order, then over the blocks by a small launch.
-constexpr int D_ROWS = 8, D_COLS = 256;
+constexpr int D_ROWS = 8, D_COLS = 256, D_BLOCKS = 4;      // blocks per SM
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, D_BLOCKS)
 linear_dpre_kernel(const T* __restrict__ dy, int64_t ld_dy, const T* __restrict__ pre, T* __restrict__ dpre, float* __restrict__ part, T* __restrict__ dbias,
                    int rows, int n, int per, int act) {
   __shared__ float s_sum[D_ROWS][D_COLS];
@@ -579,7 +579,7 @@ linear_dpre_kernel(const T* __restrict__ dy, int64_t ld_dy, const T* __restrict_
   if (c < n) {
     by_act(act, [&](auto a) {
       constexpr int ACT = decltype(a)::value;
-#pragma unroll 2
+#pragma unroll 4
       for (int r = first + rl; r < last; r += D_ROWS) {
         float g[8], x[8];
         octet_to_f32(ld_octet(dy + r * ld_dy + c), g);
@@ -770,7 +770,7 @@ static int launch_product(const hyc_linear* a, cudaStream_t st) {
 constexpr int kDpreParts = 64;      // most row ranges whose column sums are kept apart
 static int dpre_rows(int64_t rows, int n) {
   const int64_t blocks = (n + D_COLS - 1) / D_COLS;
-  int64_t parts = ((int64_t)num_sms() * 6 + blocks - 1) / blocks;      // about six blocks of 256 threads per SM
+  int64_t parts = (int64_t)num_sms() * D_BLOCKS / blocks;      // one wave
   parts = parts > kDpreParts ? kDpreParts : parts < 1 ? 1 : parts;
   int64_t per = (rows + parts - 1) / parts;
   if (rows <= 64) per = 64;      // eight rows per thread take less than the launch that adds up blocks
