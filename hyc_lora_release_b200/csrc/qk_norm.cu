@@ -393,23 +393,39 @@ static QkDivisor qk_divisor(uint32_t d) {
   return {d, (uint32_t)((((1ull << shift) - d) << 32) / d + 1), shift};
 }
 
-// Blocks for the two tensors in proportion to their heads, at most one resident wave and no more than there is work for; a token's head
-// groups are dealt to several warps where that evens out what the warps have to do.
+// How one tensor's items are cut, for `blocks` blocks: a warp's share is a whole number of items, so that small ones fill the last round, and each
+// costs about two groups more (division, angles).  Returns what the busiest warp has to do, in groups.
+static int64_t qk_cut(QkTensor& t, int tokens, int groups, int blocks) {
+  const int64_t warps = (int64_t)blocks * kQkWarps;
+  int64_t best = 0;
+  for (int i = 1; i <= 9; ++i) {
+    const int want = i <= 8 ? i : groups;      // items of a token
+    if (want > groups) continue;
+    const int per_split = (groups + want - 1) / want, splits = (groups + per_split - 1) / per_split;
+    const int64_t cost = ((int64_t)tokens * splits + warps - 1) / warps * (per_split + 2);
+    if (best == 0 || cost < best) { best = cost; t.per_split = per_split; t.splits = splits; }
+  }
+  return best;
+}
+// Blocks for the two tensors, at most one resident wave and no more than there is work for: in proportion to what their tokens cost, moved
+// by what the whole numbers of items make of it.
 static void qk_plan(QkParams& p, int group, int wave) {
-  const int per = 32 / group, heads = p.t[0].heads + p.t[1].heads;
+  const int per = 32 / group;
+  int groups[2];
+  for (int i = 0; i < 2; ++i) groups[i] = (p.t[i].heads + per - 1) / per;
+  const int even = (int)((int64_t)wave * (groups[0] + 2) / (groups[0] + groups[1] + 4)), step = wave / 32;
+  int64_t best = 0;
+  int first = even;
+  for (int i = -2; i <= 2; ++i) {
+    int blocks = even + i * step;
+    blocks = blocks < 1 ? 1 : blocks > wave - 1 ? wave - 1 : blocks;
+    const int64_t q = qk_cut(p.t[0], p.tokens, groups[0], blocks), k = qk_cut(p.t[1], p.tokens, groups[1], wave - blocks), cost = q > k ? q : k;
+    if (best == 0 || cost < best) { best = cost; first = blocks; }
+  }
   for (int i = 0; i < 2; ++i) {
     QkTensor& t = p.t[i];
-    const int groups = (t.heads + per - 1) / per;
-    int blocks = (int)((int64_t)wave * t.heads / heads);
-    if (blocks < 1) blocks = 1;
-    // a warp's share is a whole number of items: small ones fill the last round, each costs about two groups more (division, angles)
-    const int64_t warps = (int64_t)blocks * kQkWarps;
-    int64_t best = 0;
-    for (int per_split = 1; per_split <= groups; ++per_split) {
-      const int splits = (groups + per_split - 1) / per_split;
-      const int64_t cost = ((int64_t)p.tokens * splits + warps - 1) / warps * (per_split + 2);
-      if (best == 0 || cost <= best) { best = cost; t.per_split = per_split; t.splits = splits; }
-    }
+    const int blocks = i == 0 ? first : wave - first;
+    qk_cut(t, p.tokens, groups[i], blocks);
     t.by_splits = qk_divisor((uint32_t)t.splits);
     const int64_t need = ((int64_t)p.tokens * t.splits + kQkWarps - 1) / kQkWarps;
     t.blocks = (int)(need < blocks ? need : blocks);
