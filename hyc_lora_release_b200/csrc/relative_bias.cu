@@ -490,61 +490,98 @@ relbias_bwd_kernel(const __grid_constant__ RbParams p) {
     next.wait();
     a += p.cols;
     g += p.cols;
-    float dots[V], dot = 0.f;
+    // 256 columns at a time (SUB pieces, KO times): what lies before a row's end, across it or behind it is decided once for them
+    constexpr int SUB = 8 / V, KO = NV / SUB;
+    float dots[8], dot = 0.f;
 #pragma unroll
-    for (int e = 0; e < V; ++e) dots[e] = 0.f;
+    for (int e = 0; e < 8; ++e) dots[e] = 0.f;
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int cb = c0 + k * 32 * V, c = cb + lane * V;
+    for (int o = 0; o < KO; ++o) {
+      const int cb = c0 + o * 256;
       if (cb >= end) continue;           // (the whole warp, as below)
-      float fa[V], fg[V];
-      next.get(2 * k, fa);
-      next.get(2 * k + 1, fg);
-      if (cb + 32 * V <= end) {
-        mul_all(fa, fg);
-        add_all(dots, fa);
-      } else {
+      float fa[SUB][V], fg[SUB][V];
 #pragma unroll
-        for (int e = 0; e < V; ++e)
-          if (c + e < end) dots[e] = fmaf(fa[e], fg[e], dots[e]);
+      for (int j = 0; j < SUB; ++j) {
+        next.get(2 * (o * SUB + j), fa[j]);
+        next.get(2 * (o * SUB + j) + 1, fg[j]);
+        mul_all(fa[j], fg[j]);
       }
+      if (cb + 256 > end) {
+#pragma unroll
+        for (int j = 0; j < SUB; ++j)
+#pragma unroll
+          for (int e = 0; e < V; ++e) fa[j][e] = cl + (o * SUB + j) * 32 * V + e < end ? fa[j][e] : 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < SUB; ++j)
+#pragma unroll
+        for (int e = 0; e < V; ++e) dots[j * V + e] += fa[j][e];
     }
 #pragma unroll
-    for (int e = 0; e < V; ++e) dot += dots[e];
+    for (int e = 0; e < 8; ++e) dot += dots[e];
     dot = warp_sum(dot);
     if (WIDE) dot = rb_exchange(s_ex, turn, warps, p.cluster, rank, make_float2(dot, 0.f), [](float2 u, float2 v) { return make_float2(u.x + v.x, 0.f); }).x;
     // the gradient, and the diagonals' running sums: one column to the right, this row's share added
     float left = 0.f;                    // lane 0: what leaves the piece of columns before
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int cb = c0 + k * 32 * V, c = cb + lane * V;
-      float ds[V], o[V], fg[V];
-      next.get(2 * k, ds);
-      next.get(2 * k + 1, fg);
-      if (c < end_next) { next.fetch(2 * k, a + k * 32 * V); next.fetch(2 * k + 1, g + k * 32 * V); }      // (the places are free: the next row's are on their way)
+    for (int o = 0; o < KO; ++o) {
+      const int cb = c0 + o * 256;
+      float ds[SUB][V], fg[SUB][V];
+      auto to_come = [&]() {               // (the places are free: the next row's are on their way)
+#pragma unroll
+        for (int j = 0; j < SUB; ++j) {
+          const int k = o * SUB + j;
+          if (cl + k * 32 * V < end_next) { next.fetch(2 * k, a + k * 32 * V); next.fetch(2 * k + 1, g + k * 32 * V); }
+        }
+      };
+      auto store = [&]() {
+#pragma unroll
+        for (int j = 0; j < SUB; ++j) {
+          const int k = o * SUB + j;
+#pragma unroll
+          for (int e = 0; e < V; ++e) fg[j][e] = ds[j][e];
+          mul_one(fg[j], p.scale);
+          if (cl + k * 32 * V < p.cols) st_piece(dst + k * 32 * V, fg[j]);
+        }
+      };
       if (cb >= end) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) { ds[e] = 0.f; o[e] = 0.f; }
-        if (c < p.cols) st_piece(dst + k * 32 * V, o);
+        for (int j = 0; j < SUB; ++j)
+#pragma unroll
+          for (int e = 0; e < V; ++e) ds[j][e] = 0.f;
+        to_come();
+        store();
         if (p.causal) { left = 0.f; continue; }      // columns that no row so far has seen: no sums either
       } else {
-        add_one(fg, -dot);
-        mul_all(ds, fg);
-        if (cb + 32 * V > end) {
 #pragma unroll
-          for (int e = 0; e < V; ++e) ds[e] = c + e < end ? ds[e] : 0.f;
+        for (int j = 0; j < SUB; ++j) {
+          next.get(2 * (o * SUB + j), ds[j]);
+          next.get(2 * (o * SUB + j) + 1, fg[j]);
         }
+        to_come();
 #pragma unroll
-        for (int e = 0; e < V; ++e) o[e] = ds[e];
-        mul_one(o, p.scale);
-        if (c < p.cols) st_piece(dst + k * 32 * V, o);
+        for (int j = 0; j < SUB; ++j) {
+          add_one(fg[j], -dot);
+          mul_all(ds[j], fg[j]);
+        }
+        if (cb + 256 > end) {
+#pragma unroll
+          for (int j = 0; j < SUB; ++j)
+#pragma unroll
+            for (int e = 0; e < V; ++e) ds[j][e] = cl + (o * SUB + j) * 32 * V + e < end ? ds[j][e] : 0.f;
+        }
+        store();
       }
-      const float moved = __shfl_sync(0xffffffffu, acc[k][V - 1], (lane + 31) & 31);
-      const float carry = lane == 0 ? left : moved;
-      left = moved;
 #pragma unroll
-      for (int e = V - 1; e > 0; --e) acc[k][e] = acc[k][e - 1] + ds[e];
-      acc[k][0] = carry + ds[0];
+      for (int j = 0; j < SUB; ++j) {
+        const int k = o * SUB + j;
+        const float moved = __shfl_sync(0xffffffffu, acc[k][V - 1], (lane + 31) & 31);
+        const float carry = lane == 0 ? left : moved;
+        left = moved;
+#pragma unroll
+        for (int e = V - 1; e > 0; --e) acc[k][e] = acc[k][e - 1] + ds[j][e];
+        acc[k][0] = carry + ds[j][0];
+      }
     }
     if (lane == 0 && i > first) s_flush[last - i] = left;
   }
