@@ -14,13 +14,6 @@ __device__ __forceinline__ Octet<T> ld_octet(const T* p) {
   for (int i = 0; i < (int)sizeof(T) / 2; ++i) o.v[i] = reinterpret_cast<const uint4*>(p)[i];
   return o;
 }
-template <typename T>
-__device__ __forceinline__ Octet<T> zero_octet() {
-  Octet<T> o;
-#pragma unroll
-  for (int i = 0; i < (int)sizeof(T) / 2; ++i) o.v[i] = make_uint4(0u, 0u, 0u, 0u);
-  return o;
-}
 __device__ __forceinline__ float2 half2_bits_to_f32(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
 __device__ __forceinline__ uint32_t f32_to_half2_bits(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);

@@ -5,6 +5,7 @@ Every operator is checked on what the step hands it (the tolerances of its own t
 autograd on the formulas in 64 bits, in norm: a path through the step passes at most 24 roundings to bf16, each off by half a step
 (2^-8) relative to the norm, and products of random factors carry a relative error on as it is: 24 * 2^-8."""
 import math
+import threading
 
 import pytest
 import torch
@@ -140,3 +141,26 @@ def test_a_step_as_a_graph_beside_an_eager_one():
         y2, grads2, _ = _step(other, dy2, cos, sin, buckets)
     torch.cuda.current_stream().wait_stream(stream)
     assert torch.equal(y, y2) and all(torch.equal(grads[n], grads2[n]) for n in grads)
+
+
+def test_steps_of_several_threads_at_once():
+    """Each with a stream of its own: tensor memory, shared memory and workspaces are each call's own."""
+    p, dy, cos, sin, buckets = _setup(5)
+    y, grads, _ = _step(p, dy, cos, sin, buckets)
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work():
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(10):
+                y2, grads2, _ = _step(p, dy, cos, sin, buckets)
+                if not (torch.equal(y, y2) and all(torch.equal(grads[n], grads2[n]) for n in grads)):
+                    wrong.append(1)
+            stream.synchronize()
+    threads = [threading.Thread(target=work) for _ in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
