@@ -16,8 +16,8 @@
 // lane over all its heads, then per block in a fixed order, then one small launch over the blocks: the same bits on every run.
 //
 // B200, bf16, heads of 128, q and k of 32 + 8 heads: 4 x 2048 tokens forward 26 us (6.4 TB/s, 0.98 of the copy peak), backward 42 us (6.0 TB/s); 2048
-// tokens of 32 + 32 heads 14 us and 20 + 5 us.  fp32 heads of 96 18 and 26 us for 4096 tokens of 24 + 8 (0.86, 0.88).  Heads whose size is no power
-// of two leave lanes idle: 4 x 2048 tokens of 32 + 8 heads of 80 31 and 43 us (0.51, 0.56).
+// tokens of 32 + 32 heads 14 us and 20 + 5 us.  fp32 heads of 96 18 and 26 us for 4096 tokens of 24 + 8 (0.86, 0.88).  4 x
+// 2048 tokens of 32 + 8 heads of 80, six of them per warp: 25 and 42 us (0.64, 0.57; four per warp, on lanes by powers of two: 31 and 43).
 #include "elem.cuh"
 #include <type_traits>
 
@@ -46,6 +46,7 @@ struct QkTensor {
   void* out;                       // contiguous [tokens, heads, d]
   int64_t xb, xm, xh, gb, gm, gh;  // strides of x and dy: batch, token, head
   int heads;
+  int groups;                      // of heads, per token
   int splits, per_split;           // a token's head groups as `splits` items of `per_split` groups
   QkDivisor by_splits;
   int blocks;                      // blocks that work on this tensor
@@ -61,8 +62,8 @@ struct QkParams {
   float* part;                     // backward: [blocks][d] sums of the weights' gradients, q's blocks first; or null
 };
 
-// The lane's channels of a head: E adjacent ones from o1 and E from o2 on.  FULL: the head's size is 2 E times a power of two and all of it
-// is turned, so that every lane has channels, all of one kind, and partners at a distance known when this is compiled.
+// The lane's channels of a head: E adjacent ones from o1 and E from o2 on.  FULL: the head's size is 2 E G and all of it is turned,
+// so that every lane has channels, all of one kind, and partners at a distance known when this is compiled.
 template <int E, int G, bool FULL> struct QkLane {
   int first, second;
   bool is_live, is_turned;
@@ -102,22 +103,31 @@ __device__ __forceinline__ void qk_angles(const QkParams& p, int b, int m, const
   for (int e = 0; e < N; ++e) a.ns[e] = a.s[e] ^ 0x8000000080000000ull;
 }
 
+// the sum over the lanes of a head; `base`: the first of them
 template <int G>
-__device__ __forceinline__ float qk_sum(float v) {
+__device__ __forceinline__ float qk_sum(float v, int base) {
+  if constexpr ((G & (G - 1)) == 0) {
 #pragma unroll
-  for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
+    for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+  } else {
+    float sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < G; ++j) sum += __shfl_sync(0xffffffffu, v, base + j);
+    return sum;
+  }
 }
 __device__ __forceinline__ float qk_total(f32x2 v) {
   const float2 t = unpair(v);
   return t.x + t.y;
 }
 // where a warp's items lie
-struct QkItem { uint32_t token; int first, b, m; };
+struct QkItem { uint32_t token; int first, groups, b, m; };      // token, its first head group and their number; batch entry and index in it
 __device__ __forceinline__ QkItem qk_item(const QkParams& p, const QkTensor& t, uint32_t item) {
   QkItem i;
   i.token = qk_divide(item, t.by_splits);
   i.first = (int)(item - i.token * (uint32_t)t.splits) * t.per_split;
+  i.groups = min(t.per_split, t.groups - i.first);
   i.b = (int)qk_divide(i.token, p.by_seq);
   i.m = (int)(i.token - (uint32_t)i.b * (uint32_t)p.seq);
   return i;
@@ -140,7 +150,7 @@ struct QkFeed {
   const T *src, *grad;
   int64_t step, grad_step;
   uint32_t item, items, item_step, base, put, got, top;
-  int left, sub;
+  int left, todo, sub;                 // heads of the item from the lane's on; groups of the item
   __device__ __forceinline__ QkFeed(const QkParams& p_, const QkTensor& t_, const L& l_, uint32_t first, uint32_t items_, uint32_t item_step_, int sub_, uint32_t smem)
       : p(p_), t(t_), l(l_), step(PER * t_.xh), grad_step(BWD ? PER * t_.gh : 0), item(first), items(items_), item_step(item_step_),
         base(smem + threadIdx.x * 16), put(base), got(base), top(base + RING * PLACE), sub(sub_) {
@@ -152,7 +162,8 @@ struct QkFeed {
     if (item >= items) return;
     const QkItem it = qk_item(p, t, item);
     const int head0 = it.first * PER + sub;
-    left = min((it.first + t.per_split) * PER, t.heads) - head0;
+    left = sub < PER ? t.heads - head0 : 0;      // (lanes that no head belongs to: none)
+    todo = it.groups;
     src = reinterpret_cast<const T*>(t.x) + it.b * t.xb + it.m * t.xm + head0 * t.xh;
     if (BWD) grad = reinterpret_cast<const T*>(t.dy) + it.b * t.gb + it.m * t.gm + head0 * t.gh;
   }
@@ -174,7 +185,7 @@ struct QkFeed {
       src += step;
       if (BWD) grad += grad_step;
       left -= PER;
-      if (left <= -sub) { item += item_step; open(); }
+      if (--todo == 0) { item += item_step; open(); }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
     put += PLACE;
@@ -221,9 +232,9 @@ qk_norm_fwd_kernel(const __grid_constant__ QkParams p) {
     QkAngles<N> a;
     qk_angles(p, it.b, it.m, l, a);
     const int head0 = it.first * PER + sub;
-    int left = min((it.first + t.per_split) * PER, t.heads) - head0;
+    int left = sub < PER ? t.heads - head0 : 0;
     T* dst = reinterpret_cast<T*>(t.out) + (int64_t)it.token * t.heads * p.d + head0 * p.d + l.o1();
-    for (; left > -sub; left -= PER, dst += out_step) {
+    for (int group = 0; group < it.groups; ++group, left -= PER, dst += out_step) {
       f32x2 f1[N], f2[N], ss = both(0.f);
       feed.wait();
       feed.take(0, f1);
@@ -232,7 +243,7 @@ qk_norm_fwd_kernel(const __grid_constant__ QkParams p) {
       feed.send();
 #pragma unroll
       for (int e = 0; e < N; ++e) ss = fma2f(f1[e], f1[e], fma2f(f2[e], f2[e], ss));
-      const f32x2 rr = both(qk_rsqrt(fmaf(qk_sum<G>(l.live() ? qk_total(ss) : 0.f), inv_d, p.eps)));
+      const f32x2 rr = both(qk_rsqrt(fmaf(qk_sum<G>(l.live() ? qk_total(ss) : 0.f, lane - lane % G), inv_d, p.eps)));
 #pragma unroll
       for (int e = 0; e < N; ++e) {
         const f32x2 n1 = mul2f(mul2f(f1[e], rr), w1[e]), n2 = mul2f(mul2f(f2[e], rr), w2[e]);
@@ -275,9 +286,9 @@ qk_norm_bwd_kernel(const __grid_constant__ QkParams p) {
     QkAngles<N> a;
     qk_angles(p, it.b, it.m, l, a);
     const int head0 = it.first * PER + sub;
-    int left = min((it.first + t.per_split) * PER, t.heads) - head0;
+    int left = sub < PER ? t.heads - head0 : 0;
     T* dst = reinterpret_cast<T*>(t.out) + (int64_t)it.token * t.heads * p.d + head0 * p.d + l.o1();
-    for (; left > -sub; left -= PER, dst += out_step) {
+    for (int group = 0; group < it.groups; ++group, left -= PER, dst += out_step) {
       const bool ok = left > 0;
       f32x2 f1[N], f2[N], g1[N], g2[N], ss = both(0.f), sg = both(0.f);
       feed.wait();
@@ -295,8 +306,8 @@ qk_norm_bwd_kernel(const __grid_constant__ QkParams p) {
         g1[e] = u; g2[e] = v;
       }
       // dx = r g w - x r^2 mean(g w x r)
-      const float r = qk_rsqrt(fmaf(qk_sum<G>(l.live() ? qk_total(ss) : 0.f), inv_d, p.eps));
-      const float pull = qk_sum<G>(l.live() ? qk_total(sg) : 0.f) * (r * inv_d) * (r * -r);
+      const float r = qk_rsqrt(fmaf(qk_sum<G>(l.live() ? qk_total(ss) : 0.f, lane - lane % G), inv_d, p.eps));
+      const float pull = qk_sum<G>(l.live() ? qk_total(sg) : 0.f, lane - lane % G) * (r * inv_d) * (r * -r);
       const f32x2 rr = both(r), pp = both(pull);
 #pragma unroll
       for (int e = 0; e < N; ++e) {
@@ -316,10 +327,12 @@ qk_norm_bwd_kernel(const __grid_constant__ QkParams p) {
   float* s_part = reinterpret_cast<float*>(s_ring);      // [warp][channel]
 #pragma unroll
   for (int e = 0; e < N; ++e) {
+    // (lanes of the first head: the others' sums, the next head's first)
+    const f32x2 mine1 = dw1[e], mine2 = dw2[e];
 #pragma unroll
-    for (int o = G; o < 32; o <<= 1) {
-      dw1[e] = add2f(dw1[e], __shfl_xor_sync(0xffffffffu, (unsigned long long)dw1[e], o));
-      dw2[e] = add2f(dw2[e], __shfl_xor_sync(0xffffffffu, (unsigned long long)dw2[e], o));
+    for (int h = 1; h < PER; ++h) {
+      dw1[e] = add2f(dw1[e], __shfl_sync(0xffffffffu, (unsigned long long)mine1, lane % G + h * G));
+      dw2[e] = add2f(dw2[e], __shfl_sync(0xffffffffu, (unsigned long long)mine2, lane % G + h * G));
     }
     if (sub == 0 && l.live()) {
       const float2 u = unpair(dw1[e]), v = unpair(dw2[e]);
@@ -386,11 +399,13 @@ static int qk_check(const hyc_qk_norm* a, bool backward) {
 
 // Channels of a lane's piece: 16 bytes, so that the lanes of a head read whole lines; fp32 heads of more than 256 channels 32 bytes, for 32 lanes
 static int qk_piece(int type, int d) { return type == HYC_F32 && d <= 256 ? 4 : 8; }
-// lanes of a head, a power of two
+// lanes of a head: a power of two, or as many as it has pieces where more heads fit into a warp that way (five and six lanes: heads of 80 and 96
+// channels, 6 and 5 of them instead of 4)
 static int qk_group(int type, int d) {
+  const int pieces = d / (2 * qk_piece(type, d));
   int g = 1;
-  while (g < d / (2 * qk_piece(type, d))) g <<= 1;
-  return g;
+  while (g < pieces) g <<= 1;
+  return 32 / pieces > 32 / g ? pieces : g;
 }
 static QkDivisor qk_divisor(uint32_t d) {
   uint32_t shift = 0;
@@ -418,10 +433,12 @@ static void qk_plan(QkParams& p, int group, int wave) {
   const int per = 32 / group;
   int groups[2];
   for (int i = 0; i < 2; ++i) groups[i] = (p.t[i].heads + per - 1) / per;
+  // (few tokens: a warp for each group)
+  const bool each = (int64_t)p.tokens * (groups[0] + groups[1]) <= (int64_t)(wave - 1) * kQkWarps;
   const int even = (int)((int64_t)wave * (groups[0] + 2) / (groups[0] + groups[1] + 4)), step = wave / 32;
   int64_t best = 0;
   int first = even;
-  for (int i = -2; i <= 2; ++i) {
+  for (int i = -2; i <= 2 && !each; ++i) {
     int blocks = even + i * step;
     blocks = blocks < 1 ? 1 : blocks > wave - 1 ? wave - 1 : blocks;
     const int64_t q = qk_cut(p.t[0], p.tokens, groups[0], blocks), k = qk_cut(p.t[1], p.tokens, groups[1], wave - blocks), cost = q > k ? q : k;
@@ -429,8 +446,15 @@ static void qk_plan(QkParams& p, int group, int wave) {
   }
   for (int i = 0; i < 2; ++i) {
     QkTensor& t = p.t[i];
-    const int blocks = i == 0 ? first : wave - first;
-    qk_cut(t, p.tokens, groups[i], blocks);
+    int blocks = i == 0 ? first : wave - first;
+    t.groups = groups[i];
+    if (each) {
+      t.per_split = 1;
+      t.splits = groups[i];
+      blocks = wave;
+    } else {
+      qk_cut(t, p.tokens, groups[i], blocks);
+    }
     t.by_splits = qk_divisor((uint32_t)t.splits);
     const int64_t need = ((int64_t)p.tokens * t.splits + kQkWarps - 1) / kQkWarps;
     t.blocks = (int)(need < blocks ? need : blocks);
@@ -473,6 +497,11 @@ static int qk_by_type(int type, int d, int rot, F&& f) {
       switch (qk_group(type, d)) {
         case 1: return full(integral_constant<int, 1>());
         case 2: return full(integral_constant<int, 2>());
+        case 3: return full(integral_constant<int, 3>());
+        case 5: return full(integral_constant<int, 5>());
+        case 6: return full(integral_constant<int, 6>());
+        case 9: return full(integral_constant<int, 9>());
+        case 10: return full(integral_constant<int, 10>());
         case 4: return full(integral_constant<int, 4>());
         case 8: return full(integral_constant<int, 8>());
         case 16: return full(integral_constant<int, 16>());

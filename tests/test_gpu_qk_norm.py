@@ -95,6 +95,16 @@ def test_head_sizes(dtype, d, rot):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("d,rot", [(48, 48), (48, 16), (80, 32), (96, 96), (112, 112), (144, 144), (160, 96), (192, 192), (240, 240), (288, 288)])
+@pytest.mark.parametrize("hq,hk", [(1, 1), (7, 3), (24, 11)])
+def test_heads_that_share_a_warp(dtype, d, rot, hq, hk):
+    """Head sizes with any number of lanes, head counts that fill their last warp or do not."""
+    q, k, w, dy = _inputs(2, 9, hq, hk, d, DTYPES[dtype], packed=True, seed=d + hq)
+    _check(q, k, w, dy, *_tables(9, rot, torch.float32), None, rot)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("b,m,hq,hk", [(1, 1, 1, 1), (8, 1, 32, 8), (1, 257, 7, 7), (3, 333, 12, 4), (2, 1500, 32, 32), (300, 3, 5, 1)])
 @pytest.mark.parametrize("table", ["bf16", "fp32"])
 def test_sizes_and_positions(b, m, hq, hk, table):
