@@ -23,7 +23,7 @@
 //
 // B200, us, share of the copy peak, forward / backward (without the second launch, 5 us): bf16 [4,32,512,512] 29 (padding, 0.70) / 40 (0.77);
 // [1,32,2048,2048] 90 (0.91) / 137 (0.90), causal 79 (0.78) / 105 (0.78); [2,32,696,696] causal 35 (0.41) / 31 (0.61); fp32 [4,16,1000,1000] 87 (0.90) /
-// 115 (1.0); fp16 [2,32,1002,1002] 56 (0.70) / 69 (0.85), [2,32,1001,1001] causal 68 (0.43) / 81 (0.48): single elements per access cost instructions.
+// 115 (1.0); fp16 [2,32,1002,1002] 54 (0.73) / 69 (0.85), [2,32,1001,1001] causal 64 (0.46) / 81 (0.48): single elements per access cost instructions.
 // Forward is bound by instruction issue (15 per element, exponentials a third of their unit), backward by the latency of its rows.
 #include "elem.cuh"
 #include <type_traits>
@@ -337,30 +337,40 @@ relbias_fwd_kernel(const __grid_constant__ RbParams p) {
         add_all(f[k], mk);
       }
     }
+    // what lies across the row's end or behind it is decided once for 256 columns (per piece: [4,3,1470,1707] 68 us, so 53)
+    constexpr int SUB = 8 / V;
 #pragma unroll
-    for (int k = 0; k < NA; ++k) {
-      const int cb = c0 + k * 32 * V, c = cb + lane * V;
-      if (cb + 32 * V > end) {           // (else all of the warp's columns count)
+    for (int o = 0; o < NA; o += SUB) {
+      if (c0 + (o + SUB) * 32 * V > end) {      // (else all of the warp's columns count)
 #pragma unroll
-        for (int e = 0; e < V; ++e) f[k][e] = c + e < end ? f[k][e] : -INFINITY;
+        for (int k = o; k < o + SUB; ++k)
+#pragma unroll
+          for (int e = 0; e < V; ++e) f[k][e] = cl + k * 32 * V + e < end ? f[k][e] : -INFINITY;
       }
 #pragma unroll
-      for (int e = 0; e < V; ++e) tops[(k * V + e) & 3] = fmaxf(tops[(k * V + e) & 3], f[k][e]);
+      for (int k = o; k < o + SUB; ++k)
+#pragma unroll
+        for (int e = 0; e < V; ++e) tops[(k * V + e) & 3] = fmaxf(tops[(k * V + e) & 3], f[k][e]);
     }
     m = warp_max(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])));
     const float mm = m == -INFINITY ? 0.f : m;      // nothing counts: 2^-inf = 0 everywhere
-    float sums[V], sum = 0.f;
+    float sums[V < 4 ? 4 : V], sum = 0.f;
 #pragma unroll
-    for (int e = 0; e < V; ++e) sums[e] = 0.f;
+    for (int e = 0; e < (V < 4 ? 4 : V); ++e) sums[e] = 0.f;
 #pragma unroll
     for (int k = 0; k < NA; ++k) {
       add_one(f[k], -mm);
 #pragma unroll
       for (int e = 0; e < V; ++e) f[k][e] = exp2_neg(f[k][e]);
-      add_all(sums, f[k]);
+      if constexpr (V == 8) {
+        add_all(sums, f[k]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) sums[(k * V + e) & 3] += f[k][e];
+      }
     }
 #pragma unroll
-    for (int e = 0; e < V; ++e) sum += sums[e];
+    for (int e = 0; e < (V < 4 ? 4 : V); ++e) sum += sums[e];
     sum = warp_sum(sum);
     float factor;
     if (WIDE) {
@@ -371,14 +381,18 @@ relbias_fwd_kernel(const __grid_constant__ RbParams p) {
       factor = sum == 0.f ? 0.f : __fdividef(1.f, sum);        // a row that nothing is visible to: zeros
     }
 #pragma unroll
-    for (int k = 0; k < NA; ++k) {
-      const int cb = c0 + k * 32 * V, c = cb + lane * V;
-      mul_one(f[k], factor);
-      if (cb + 32 * V > end) {
+    for (int o = 0; o < NA; o += SUB) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) f[k][e] = c + e < end ? f[k][e] : 0.f;      // (zero in a row that became NaN, too)
+      for (int k = o; k < o + SUB; ++k) mul_one(f[k], factor);
+      if (c0 + (o + SUB) * 32 * V > end) {
+#pragma unroll
+        for (int k = o; k < o + SUB; ++k)
+#pragma unroll
+          for (int e = 0; e < V; ++e) f[k][e] = cl + k * 32 * V + e < end ? f[k][e] : 0.f;      // (zero in a row that became NaN, too)
       }
-      if (c < p.cols) st_piece(dst + k * 32 * V, f[k]);
+#pragma unroll
+      for (int k = o; k < o + SUB; ++k)
+        if (cl + k * 32 * V < p.cols) st_piece(dst + k * 32 * V, f[k]);
     }
 #pragma unroll
     for (int k = NA; k < NV; ++k) {      // columns behind the row's end
@@ -393,7 +407,7 @@ relbias_fwd_kernel(const __grid_constant__ RbParams p) {
     }
     };
     // (not where warps meet: all of them have to be on the same line)
-    if (!WIDE && NV >= 4 && end <= SPAN / 2) row(std::integral_constant<int, NV >= 4 ? NV / 2 : NV>());
+    if (!WIDE && SPAN >= 512 && end <= SPAN / 2) row(std::integral_constant<int, SPAN >= 512 ? NV / 2 : NV>());
     else row(std::integral_constant<int, NV>());
   }
 }
