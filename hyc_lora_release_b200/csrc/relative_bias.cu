@@ -19,11 +19,13 @@
 // running sum of each diagonal moves one column to the right: within a lane's V columns that is an operand of the addition, between
 // lanes one shuffle per V elements, and what leaves the warp's last column is put aside in shared memory.  After the last row the
 // sums of SPAN + R - 1 diagonals are there, and each bucket's are added up: no atomics, the same bits on every run.  A small
-// second launch adds the warps' sums per head (in 64 bits: whole maps that nearly cancel).
+// second launch adds the warps' sums per head.  Buckets hold long ranges whose sums nearly cancel, so from the diagonals on all sums are in
+// 64 bits, and so is a row's product sum where warps share the row (few rows: nothing averages out; in 32 bits throughout the
+// table's gradient of single tokens was up to 15 times as far off as the formula's in 32 bits with sums in 64; 1 to 2 us more, 41 -> 42.5).
 //
-// B200, us, share of the copy peak, forward / backward (without the second launch, 5 us): bf16 [4,32,512,512] 29 (padding, 0.70) / 40 (0.77);
-// [1,32,2048,2048] 90 (0.91) / 137 (0.90), causal 79 (0.78) / 105 (0.78); [2,32,696,696] causal 35 (0.41) / 31 (0.61); fp32 [4,16,1000,1000] 87 (0.90) /
-// 115 (1.0); fp16 [2,32,1002,1002] 54 (0.73) / 69 (0.85), [2,32,1001,1001] causal 64 (0.46) / 81 (0.48): single elements per access cost instructions.
+// B200, us, share of the copy peak, forward / backward (without the second launch, 5 us): bf16 [4,32,512,512] 29 (padding, 0.70) / 42 (0.73);
+// [1,32,2048,2048] 90 (0.91) / 139 (0.89), causal 79 (0.78) / 106 (0.77); [2,32,696,696] causal 35 (0.41) / 32 (0.59); fp32 [4,16,1000,1000] 87 (0.90) /
+// 117 (1.0); fp16 [2,32,1002,1002] 54 (0.73) / 69 (0.85), [2,32,1001,1001] causal 64 (0.46) / 82 (0.48): single elements per access cost instructions.
 // Forward is bound by instruction issue (15 per element, exponentials a third of their unit), backward by the latency of its rows.
 #include "elem.cuh"
 #include <type_traits>
@@ -39,7 +41,7 @@ constexpr int kRbMaxCluster = 8;
 struct RbParams {
   const void *x, *grad, *table, *mask;
   void* out;
-  float* part;                           // backward: [unit][buckets]
+  double* part;                          // backward: [unit][buckets]
   int64_t mask_b, mask_h, mask_row;
   int64_t units;                         // backward: warps (narrow), blocks or clusters (wide) with rows
   int heads, n, cols, q_offset;
@@ -79,7 +81,8 @@ __device__ __forceinline__ float warp_max(float v) {      // (a NaN among the va
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
   return r;
 }
-__device__ __forceinline__ float warp_sum(float v) {
+template <typename F>
+__device__ __forceinline__ F warp_sum(F v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
@@ -161,27 +164,32 @@ __device__ __forceinline__ void mul_all(float (&x)[V], const float (&b)[V]) {
   }
 }
 
-// ---- exchange between the warps that share a row: every warp gives a pair and receives all of them combined.  `turn` alternates,
+// ---- exchange between the warps that share a row: every warp gives a value of 8 bytes and receives all of them combined.  `turn` alternates,
 // so that the next row's values cannot meet this one's readers.
+template <typename E>
 struct RbExchange {
-  float2 warp[2][kRbMaxWarps];
-  float2 block[2][kRbMaxCluster];
+  E warp[2][kRbMaxWarps];
+  E block[2][kRbMaxCluster];
 };
 __device__ __forceinline__ void rb_cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void rb_put(float2* slot, int rank, float2 v) {      // into block `rank` of the cluster
+__device__ __forceinline__ void rb_put(void* slot, int rank, float2 v) {      // into block `rank` of the cluster
   uint32_t at;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(slot)), "r"(rank));
   asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(at), "f"(v.x), "f"(v.y) : "memory");
 }
-template <typename F>
-__device__ __forceinline__ float2 rb_exchange(RbExchange& ex, int turn, int warps, int cluster, int rank, float2 mine, F&& join) {
+__device__ __forceinline__ void rb_put(void* slot, int rank, double v) {
+  const long long bits = __double_as_longlong(v);
+  rb_put(slot, rank, make_float2(__int_as_float((int)bits), __int_as_float((int)(bits >> 32))));
+}
+template <typename E, typename F>
+__device__ __forceinline__ E rb_exchange(RbExchange<E>& ex, int turn, int warps, int cluster, int rank, E mine, F&& join) {
   const int warp = threadIdx.x >> 5;
   if ((threadIdx.x & 31) == 0) ex.warp[turn][warp] = mine;
   __syncthreads();
-  float2 all = ex.warp[turn][0];
+  E all = ex.warp[turn][0];
   for (int w = 1; w < warps; ++w) all = join(all, ex.warp[turn][w]);
   if (cluster == 1) return all;
   if ((int)threadIdx.x < cluster) rb_put(&ex.block[turn][rank], (int)threadIdx.x, all);
@@ -221,7 +229,7 @@ relbias_fwd_kernel(const __grid_constant__ RbParams p) {
   extern __shared__ __align__(16) float s_mem[];
   __shared__ int s_edges[kRbMaxSide];
   __shared__ float s_table[2 * kRbMaxSide];
-  __shared__ RbExchange s_ex;
+  __shared__ RbExchange<float2> s_ex;
   constexpr int SPAN = 32 * V * NV;
   const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), warps = blockDim.x >> 5;
   const int rank = WIDE ? (int)(blockIdx.x % (unsigned)p.cluster) : 0;
@@ -469,7 +477,7 @@ __global__ void __launch_bounds__(WIDE ? 32 * kRbMaxWarps : 32 * kRbBwdWarps, WI
 relbias_bwd_kernel(const __grid_constant__ RbParams p) {
   extern __shared__ __align__(16) float s_diag_all[];
   __shared__ int s_edges[kRbMaxSide];
-  __shared__ RbExchange s_ex;
+  __shared__ RbExchange<double> s_ex;
   constexpr int SPAN = 32 * V * NV;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const int rank = WIDE ? (int)(blockIdx.x % (unsigned)p.cluster) : 0;
@@ -511,7 +519,7 @@ relbias_bwd_kernel(const __grid_constant__ RbParams p) {
     g += p.cols;
     // 256 columns at a time (SUB pieces, KO times): what lies before a row's end, across it or behind it is decided once for them
     constexpr int SUB = 8 / V, KO = NV / SUB;
-    float dots[8], dot = 0.f;
+    float dots[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) dots[e] = 0.f;
 #pragma unroll
@@ -537,9 +545,15 @@ relbias_bwd_kernel(const __grid_constant__ RbParams p) {
         for (int e = 0; e < V; ++e) dots[j * V + e] += fa[j][e];
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) dot += dots[e];
-    dot = warp_sum(dot);
-    if (WIDE) dot = rb_exchange(s_ex, turn, warps, p.cluster, rank, make_float2(dot, 0.f), [](float2 u, float2 v) { return make_float2(u.x + v.x, 0.f); }).x;
+    for (int o = 4; o > 1; o >>= 1)
+#pragma unroll
+      for (int e = 0; e < o; ++e) dots[e] += dots[e + o];
+    float dot;
+    if constexpr (WIDE) {                // (few rows: what a row's sum is off by averages out in no bucket)
+      dot = (float)rb_exchange(s_ex, turn, warps, p.cluster, rank, warp_sum((double)dots[0] + (double)dots[1]), [](double u, double v) { return u + v; });
+    } else {
+      dot = warp_sum(dots[0] + dots[1]);
+    }
     // the gradient, and the diagonals' running sums: one column to the right, this row's share added
     float left = 0.f;                    // lane 0: what leaves the piece of columns before
 #pragma unroll
@@ -580,8 +594,13 @@ relbias_bwd_kernel(const __grid_constant__ RbParams p) {
         to_come();
 #pragma unroll
         for (int j = 0; j < SUB; ++j) {
-          add_one(fg[j], -dot);
-          mul_all(ds[j], fg[j]);
+          if constexpr (sizeof(T) == 2) {      // a g is exact: one rounding
+            mul_all(fg[j], ds[j]);
+            fma_all(ds[j], -dot, fg[j]);
+          } else {
+            add_one(fg[j], -dot);
+            mul_all(ds[j], fg[j]);
+          }
         }
         if (cb + 256 > end) {
 #pragma unroll
@@ -612,8 +631,19 @@ relbias_bwd_kernel(const __grid_constant__ RbParams p) {
   __syncwarp();
   // the sum of the diagonal at distance dmin + x: s_diag[x], behind the warp's columns s_flush[x - SPAN]
   auto diagonal = [&](int x) { return x < SPAN ? s_diag[x] : s_flush[x - SPAN]; };
+  // .. of every step-th distance from..to, in 64 bits: long ranges nearly cancel
+  auto every = [&](int from, int to, int step) {
+    double sum = 0.0;
+    for (int x = from; x <= to; x += 4 * step) {
+      float v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = x + j * step <= to ? diagonal(x + j * step) : 0.f;
+      sum += ((double)v[0] + (double)v[1]) + ((double)v[2] + (double)v[3]);
+    }
+    return sum;
+  };
   const int dmin = c0 - last - p.q_offset, dmax = dmin + SPAN - 1 + (last - first);
-  float* part = p.part + ((WIDE ? unit * p.cluster * warps + rank * warps + warp : unit)) * p.buckets;
+  double* part = p.part + ((WIDE ? unit * p.cluster * warps + rank * warps + warp : unit)) * p.buckets;
   // short ranges by a lane each, long ones by the warp
   for (int k0 = 0; k0 < p.buckets; k0 += 32) {
     const int k = k0 + lane;
@@ -621,14 +651,10 @@ relbias_bwd_kernel(const __grid_constant__ RbParams p) {
     if (k < p.buckets) rb_range(p, s_edges, k, from, to);
     from = max(from, dmin); to = min(to, dmax);
     const bool wide_range = to - from >= 48;
-    float sum = 0.f;
-    if (!wide_range)
-      for (int d = from; d <= to; ++d) sum += diagonal(d - dmin);
+    double sum = wide_range ? 0.0 : every(from - dmin, to - dmin, 1);
     for (unsigned left = __ballot_sync(0xffffffffu, wide_range); left != 0u; left &= left - 1u) {
       const int l = __ffs(left) - 1, lo = __shfl_sync(0xffffffffu, from, l), hi = __shfl_sync(0xffffffffu, to, l);
-      float v = 0.f;
-      for (int d = lo + lane; d <= hi; d += 32) v += diagonal(d - dmin);
-      v = warp_sum(v);
+      const double v = warp_sum(every(lo + lane - dmin, hi - dmin, 32));
       if (lane == l) sum = v;
     }
     if (k < p.buckets) part[k] = sum;
@@ -637,7 +663,7 @@ relbias_bwd_kernel(const __grid_constant__ RbParams p) {
 
 // table[k, head]: the units' sums of a head, 32 buckets per block
 __global__ void __launch_bounds__(1024)
-relbias_table_kernel(const float* __restrict__ part, int batch, int heads, int per_map, int buckets, float* __restrict__ table) {
+relbias_table_kernel(const double* __restrict__ part, int batch, int heads, int per_map, int buckets, float* __restrict__ table) {
   __shared__ double s_sum[32][33];
   pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, h = (int)blockIdx.x, k = (int)blockIdx.y * 32 + lane;
@@ -647,7 +673,7 @@ relbias_table_kernel(const float* __restrict__ part, int batch, int heads, int p
 #pragma unroll 4
     for (uint32_t u = warp; u < units; u += 32) {
       const uint32_t b = u / (uint32_t)per_map;
-      sum += (double)part[((int64_t)(b * heads + h) * per_map + (u - b * per_map)) * buckets + k];
+      sum += part[((int64_t)(b * heads + h) * per_map + (u - b * per_map)) * buckets + k];
     }
   }
   s_sum[warp][lane] = sum;
@@ -834,7 +860,7 @@ extern "C" HYC_API int hyc_softmax_relative_bias_fwd(const hyc_relative_bias* a,
 
 extern "C" HYC_API size_t hyc_softmax_relative_bias_workspace_bytes(const hyc_relative_bias* a) {
   if (rb_check(a, true) != HYC_OK || a->batch * a->n == 0) return 0;
-  return (size_t)rb_units(a, rb_plan(a, true)).sums * (size_t)(a->both ? 2 * a->side : a->side) * sizeof(float);
+  return (size_t)rb_units(a, rb_plan(a, true)).sums * (size_t)(a->both ? 2 * a->side : a->side) * sizeof(double);
 }
 
 extern "C" HYC_API int hyc_softmax_relative_bias_bwd(const hyc_relative_bias* a, float* dtable, void* workspace, size_t workspace_bytes, void* stream) {
@@ -848,10 +874,10 @@ extern "C" HYC_API int hyc_softmax_relative_bias_bwd(const hyc_relative_bias* a,
   if (a->batch * a->n != 0) {
     r = rb_plan(a, true);
     u = rb_units(a, r);
-    if (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < (size_t)u.sums * (size_t)buckets * sizeof(float)) return HYC_ERR_WORKSPACE;
+    if (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < (size_t)u.sums * (size_t)buckets * sizeof(double)) return HYC_ERR_WORKSPACE;
     RbParams p;
     rb_fill(p, a, r);
-    p.part = (float*)workspace;
+    p.part = (double*)workspace;
     p.rows_per = u.rows_per; p.chunks = u.chunks; p.units = u.units;
     const int64_t blocks = r.wide ? u.units * r.cluster : (u.units + kRbBwdWarps - 1) / kRbBwdWarps;
     const int rl = rb_by_plan(a->type, r, [&](auto elem, auto v, auto nv, auto wide) -> int {
@@ -863,7 +889,7 @@ extern "C" HYC_API int hyc_softmax_relative_bias_bwd(const hyc_relative_bias* a,
     if (rl != HYC_OK) return rl;
   }
   const int per_map = u.chunks * (r.wide ? r.warps * r.cluster : 1);
-  launch_pdl(relbias_table_kernel, dim3((unsigned)a->heads, (unsigned)((buckets + 31) / 32)), dim3(1024), 0, (cudaStream_t)stream, (const float*)workspace,
+  launch_pdl(relbias_table_kernel, dim3((unsigned)a->heads, (unsigned)((buckets + 31) / 32)), dim3(1024), 0, (cudaStream_t)stream, (const double*)workspace,
              u.units > 0 ? (int)a->batch : 0, a->heads, per_map, buckets, dtable);
   HYC_CHECK_LAUNCH();
   return HYC_OK;

@@ -333,6 +333,30 @@ def test_offsets_beyond_32_bits():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("b,h,n,cols", [(4, 16, 1, 1670), (3, 1, 3, 1277), (8, 12, 1, 4000), (2, 3, 1, 13384)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_table_gradient_of_few_rows(b, h, n, cols, dtype):
+    """A bucket that holds nearly all of a row, whose sum nearly cancels.  In units of 2^-24: one rounding per element (a g is exact in
+    fp32), the row's product sum off by its own rounding and by at most 3 + 2 additions of a lane before 64 bits, and the result's."""
+    from hyc_lora_release_b200.operators.relative_bias_kernels import RelativeBuckets, softmax_backward_relative_bias
+    buckets, offset = RelativeBuckets(8, 64, False), cols - n
+    g = torch.Generator(device=DEV).manual_seed(cols)
+    dt = DTYPES[dtype]
+    a = torch.softmax(torch.randn(b, h, n, cols, generator=g, device=DEV) * 1.5, -1)
+    a = a.masked_fill(~visible(n, cols, True, offset), 0.0).to(dt)
+    grad = (torch.randn(b, h, n, cols, generator=g, device=DEV) * 0.05).to(dt)
+    _, got = softmax_backward_relative_bias(a, grad, 0.125, buckets, causal=True, q_offset=offset)
+    x = a.double()
+    prod = x * grad.double()
+    dot, mag = prod.sum(-1, keepdim=True), prod.abs().sum(-1, keepdim=True)
+    ds = x * (grad.double() - dot)
+    err = ds.abs() + x * (dot.abs() + 5 * mag)
+    hit = torch.nn.functional.one_hot(bucket_index(buckets, n, cols, offset), 8).double()
+    want, bound = (torch.einsum("bhij,ijk->kh", v, hit) for v in (ds, err))
+    assert bool(((got.double() - want).abs() <= 2.0 ** -24 * (bound + want.abs())).all())
+
+
+@pytest.mark.gpu
 def test_gradients_against_differences():
     """Central differences of the 64-bit formula along one direction of scores and table (truncation of order step^2)."""
     from hyc_lora_release_b200.operators import relative_bias_kernels as rb
