@@ -19,9 +19,9 @@
 // running sum of each diagonal moves one column to the right: within a lane's V columns that is an operand of the addition, between
 // lanes one shuffle per V elements, and what leaves the warp's last column is put aside in shared memory.  After the last row the
 // sums of SPAN + R - 1 diagonals are there, and each bucket's are added up: no atomics, the same bits on every run.  A small
-// second launch adds the warps' sums per head.  Buckets hold long ranges whose sums nearly cancel, so from the diagonals on all sums are in
-// 64 bits, and so is a row's product sum where warps share the row (few rows: nothing averages out; in 32 bits throughout the
-// table's gradient of single tokens was up to 15 times as far off as the formula's in 32 bits with sums in 64; 1 to 2 us more, 41 -> 42.5).
+// second launch adds the warps' sums per head, in 64 bits.  Buckets hold long ranges whose sums nearly cancel: where warps share a row (few
+// rows, nothing averages out) the row's product sum and the buckets' are in 64 bits too (in 32 the table's gradient of single tokens was
+// up to 15 times as far off as the formula's in 32 bits with sums in 64; everywhere it would cost 2 to 7 %, and there rows average it out).
 //
 // B200, us, share of the copy peak, forward / backward (without the second launch, 5 us): bf16 [4,32,512,512] 29 (padding, 0.70) / 42 (0.73);
 // [1,32,2048,2048] 90 (0.91) / 139 (0.89), causal 79 (0.78) / 106 (0.77); [2,32,696,696] causal 35 (0.41) / 32 (0.59); fp32 [4,16,1000,1000] 87 (0.90) /
@@ -631,14 +631,15 @@ relbias_bwd_kernel(const __grid_constant__ RbParams p) {
   __syncwarp();
   // the sum of the diagonal at distance dmin + x: s_diag[x], behind the warp's columns s_flush[x - SPAN]
   auto diagonal = [&](int x) { return x < SPAN ? s_diag[x] : s_flush[x - SPAN]; };
-  // .. of every step-th distance from..to, in 64 bits: long ranges nearly cancel
+  // .. of every step-th distance from..to: long ranges nearly cancel, in 64 bits where nothing averages out (few rows)
+  typedef typename std::conditional<WIDE, double, float>::type Sum;
   auto every = [&](int from, int to, int step) {
-    double sum = 0.0;
+    Sum sum = 0;
     for (int x = from; x <= to; x += 4 * step) {
       float v[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[j] = x + j * step <= to ? diagonal(x + j * step) : 0.f;
-      sum += ((double)v[0] + (double)v[1]) + ((double)v[2] + (double)v[3]);
+      sum += ((Sum)v[0] + (Sum)v[1]) + ((Sum)v[2] + (Sum)v[3]);
     }
     return sum;
   };
@@ -651,10 +652,10 @@ relbias_bwd_kernel(const __grid_constant__ RbParams p) {
     if (k < p.buckets) rb_range(p, s_edges, k, from, to);
     from = max(from, dmin); to = min(to, dmax);
     const bool wide_range = to - from >= 48;
-    double sum = wide_range ? 0.0 : every(from - dmin, to - dmin, 1);
+    Sum sum = wide_range ? (Sum)0 : every(from - dmin, to - dmin, 1);
     for (unsigned left = __ballot_sync(0xffffffffu, wide_range); left != 0u; left &= left - 1u) {
       const int l = __ffs(left) - 1, lo = __shfl_sync(0xffffffffu, from, l), hi = __shfl_sync(0xffffffffu, to, l);
-      const double v = warp_sum(every(lo + lane - dmin, hi - dmin, 32));
+      const Sum v = warp_sum(every(lo + lane - dmin, hi - dmin, 32));
       if (lane == l) sum = v;
     }
     if (k < p.buckets) part[k] = sum;
