@@ -6,7 +6,8 @@
 // All three products are C[r, c] = sum_k A[r, k] B[c, k] with operands whose contraction index is either adjacent in memory (K-major) or
 // not (MN-major: W for dx, both operands for dW): no operand is copied or transposed.  bf16 or fp16 operands, fp32 accumulators in tensor
 // memory, one rounding at the store.  dpre is rounded to 16 bits before its two products, as tensor-core operands are: its error, half a
-// step per element, averages out in the sums, which carry about 1.4 times the error of their own rounding.
+// step per element, averages out in the sums, which carry about 1.4 times the error of their own rounding
+// (up to 1.5 with one to four tokens); a second product with what the rounding took would double the work.
 //
 // Two kernels, both fed by TMA (128-byte swizzle, 64-wide k-blocks; what lies outside of an operand arrives as zero, so that any number of
 // rows and any multiple of 8 columns is right), every wait bounded (hyc_linear_status):
