@@ -584,7 +584,8 @@ relbias_bwd_kernel(const __grid_constant__ RbParams p) {
           for (int e = 0; e < V; ++e) ds[j][e] = 0.f;
         to_come();
         store();
-        if (p.causal) { left = 0.f; continue; }      // columns that no row so far has seen: no sums either
+        // columns that no row so far has seen: no sums either.  (Rows that lie behind the last column all end with it: their sums move on.)
+        if (p.causal && end < p.cols) { left = 0.f; continue; }
       } else {
 #pragma unroll
         for (int j = 0; j < SUB; ++j) {

@@ -399,3 +399,22 @@ def test_empty_and_refusals():
             call()
     with pytest.raises(RuntimeError, match="different devices|only on CUDA"):
         fwd(table=table.cpu())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,b,h,n,cols,offset", [
+    ("bf16", 2, 20, 900, 760, 0), ("bf16", 2, 20, 900, 768, 0), ("fp16", 2, 16, 1500, 1280, 0), ("bf16", 1, 20, 1700, 1536, 0), ("bf16", 1, 16, 2000, 1792, 0),
+    ("bf16", 2, 20, 700, 768, 400), ("bf16", 2, 20, 300, 1536, 2000), ("fp32", 2, 16, 900, 768, 0), ("bf16", 2, 20, 900, 766, 0), ("fp16", 2, 20, 900, 767, 3),
+    ("bf16", 1, 20, 300, 4864, 4864), ("fp16", 1, 20, 400, 4870, 4600)])
+def test_causal_rows_behind_the_last_column(dtype, b, h, n, cols, offset):
+    """Rows whose own position lies behind the map's last column see all of it, and the diagonals' sums leave the columns on the right:
+    columns that end at or close to a block of 256 inside a warp's span, more rows than columns, and keys that all lie behind."""
+    from hyc_lora_release_b200.operators.relative_bias_kernels import RelativeBuckets, softmax_backward_relative_bias
+    buckets = RelativeBuckets(32, 128, False)
+    g = torch.Generator(device=DEV).manual_seed(cols)
+    see = visible(n, cols, True, offset)
+    x = torch.randn(b, h, n, cols, generator=g, device=DEV).masked_fill(~see, -math.inf)
+    a, grad = torch.softmax(x, -1).to(DTYPES[dtype]), torch.randn(b, h, n, cols, generator=g, device=DEV).to(DTYPES[dtype])
+    ds, dt = softmax_backward_relative_bias(a, grad, 0.125, buckets, causal=True, q_offset=offset)
+    want, err, want_t, err_t = plain_backward(a, grad, 0.125, buckets, True, offset)
+    assert grad_close(ds, want, err) and grad_close(dt, want_t, err_t)
