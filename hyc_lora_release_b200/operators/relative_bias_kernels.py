@@ -36,7 +36,7 @@ class RelativeBuckets:
                     low = r + 1
             edges.append(low)
         self.num_buckets, self.max_distance, self.bidirectional = num_buckets, max_distance, bool(bidirectional)
-        self.edges = torch.tensor(edges, dtype=torch.int32)
+        self.edges = torch.tensor(edges, dtype=torch.int32, device="cpu")
 
 
 def softmax_forward_relative_bias(scores, scale, table, buckets, attention_mask=None, causal=False, q_offset=0, inplace=False):

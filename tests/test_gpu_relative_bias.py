@@ -418,3 +418,11 @@ def test_causal_rows_behind_the_last_column(dtype, b, h, n, cols, offset):
     ds, dt = softmax_backward_relative_bias(a, grad, 0.125, buckets, causal=True, q_offset=offset)
     want, err, want_t, err_t = plain_backward(a, grad, 0.125, buckets, True, offset)
     assert grad_close(ds, want, err) and grad_close(dt, want_t, err_t)
+
+
+def test_buckets_made_where_another_device_is_the_default():
+    """A model that is built under a device's context: the edges are host data all the same."""
+    from hyc_lora_release_b200.operators.relative_bias_kernels import RelativeBuckets
+    with torch.device("meta"):
+        buckets = RelativeBuckets(32, 128, True)
+    assert buckets.edges.device.type == "cpu" and torch.equal(buckets.edges, RelativeBuckets(32, 128, True).edges)
