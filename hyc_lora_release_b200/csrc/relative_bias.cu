@@ -87,18 +87,21 @@ __device__ __forceinline__ F warp_sum(F v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-// Exponents are kept times log2(e), so that an exponential is one subtraction and one instruction (two units in the last place; below
-// 2^-126 it is 0).
-constexpr float kLog2e = 1.4426950408889634f;
+// Exponents are kept times log2(e) / 256, so that an exponential is one fused multiply-add and one instruction (two units in the last place;
+// below 2^-126 it is 0), and scores, biases and masks up to the ends of fp32's range stay finite and keep their order: only what is -infinity
+// counts as nothing.
+constexpr float kSteps = 256.f, kUnit = 1.4426950408889634f / kSteps;
 __device__ __forceinline__ float exp2_neg(float v) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
-// a mask's value times log2(e); where that is beyond fp32 as it is: the type's lowest value must not become -infinity
-__device__ __forceinline__ float mask_log2e(float m) {
-  const float v = m * kLog2e;
-  return v < -3.402823466e38f ? m : v;
+// 2^(kSteps (x - top)) is exp2_neg(x s + b): the product is exact, so that the largest element gives 1.  Where kSteps top is beyond fp32,
+// two exponents are equal or so far apart that a quarter of the difference gives 0 as well.
+struct Exponents { float s, b; };
+__device__ __forceinline__ Exponents exponents(float top) {
+  const float s = fabsf(top) > 1e36f ? 0.25f : kSteps;
+  return {s, -top * s};
 }
 
 // ---- two fp32 operations per instruction, over the V values of a piece
@@ -131,6 +134,13 @@ __device__ __forceinline__ void add_all(float (&x)[V], const float (&b)[V]) {
       halves(r, x[e], x[e + 1]);
     }
   }
+}
+template <int V>
+__device__ __forceinline__ void fma_one(float (&x)[V], float s, float b) {
+  float v[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) v[e] = b;
+  fma_all(x, s, v);
 }
 template <int V>
 __device__ __forceinline__ void add_one(float (&x)[V], float b) {
@@ -202,7 +212,7 @@ __device__ __forceinline__ E rb_exchange(RbExchange<E>& ex, int turn, int warps,
 __device__ __forceinline__ float2 join_softmax(float2 a, float2 b) {
   const float m = fmaxf(a.x, b.x);
   if (m == -INFINITY) return make_float2(m, a.y + b.y);
-  return make_float2(m, a.y * exp2_neg(a.x - m) + b.y * exp2_neg(b.x - m));
+  return make_float2(m, a.y * exp2_neg((a.x - m) * kSteps) + b.y * exp2_neg((b.x - m) * kSteps));
 }
 
 // the bias table, spread for lanes eight columns apart so that they meet in no bank
@@ -256,10 +266,10 @@ relbias_fwd_kernel(const __grid_constant__ RbParams p) {
     for (int k = 0; k < NV; ++k)
       if (cl + k * 32 * V < end) ld_piece(src + k * 32 * V, raw[k]);
   }
-  for (int i = threadIdx.x; i < p.buckets; i += blockDim.x) s_table[i] = ld_any(p.table, (int64_t)i * p.heads + h, p.table_type) * kLog2e;
+  for (int i = threadIdx.x; i < p.buckets; i += blockDim.x) s_table[i] = ld_any(p.table, (int64_t)i * p.heads + h, p.table_type) * kUnit;
   if (p.mask_staged) {
     const int64_t at = b * p.mask_b + h * p.mask_h;
-    for (int i = threadIdx.x; i < p.mask_staged && block_c0 + i < p.cols; i += blockDim.x) s_mask[i] = mask_log2e(ld_any(p.mask, at + block_c0 + i, p.mask_type));
+    for (int i = threadIdx.x; i < p.mask_staged && block_c0 + i < p.cols; i += blockDim.x) s_mask[i] = ld_any(p.mask, at + block_c0 + i, p.mask_type) * kUnit;
   }
   __syncthreads();
   // the bias: of every distance that the block meets, from its first column and last row on; compact: of every distance up to the last edge
@@ -273,7 +283,7 @@ relbias_fwd_kernel(const __grid_constant__ RbParams p) {
   }
   __syncthreads();
   if (WIDE && p.cluster > 1) rb_cluster_sync();      // the other blocks have started: their shared memory may be written
-  const float scale = p.scale * kLog2e;
+  const float scale = p.scale * kUnit;
   const float* my_mask = s_mask + (cl - block_c0);
   int turn = 0;
   for (int i = first; i < last; ++i, turn ^= 1, dst += p.cols) {
@@ -340,8 +350,7 @@ relbias_fwd_kernel(const __grid_constant__ RbParams p) {
 #pragma unroll
           for (int e = 0; e < V; ++e) mk[e] = ld_any(p.mask, at + k * 32 * V + e, p.mask_type);
         }
-#pragma unroll
-        for (int e = 0; e < V; ++e) mk[e] = mask_log2e(mk[e]);
+        mul_one(mk, kUnit);
         add_all(f[k], mk);
       }
     }
@@ -361,13 +370,13 @@ relbias_fwd_kernel(const __grid_constant__ RbParams p) {
         for (int e = 0; e < V; ++e) tops[(k * V + e) & 3] = fmaxf(tops[(k * V + e) & 3], f[k][e]);
     }
     m = warp_max(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])));
-    const float mm = m == -INFINITY ? 0.f : m;      // nothing counts: 2^-inf = 0 everywhere
+    const Exponents ex = exponents(m == -INFINITY ? 0.f : m);      // nothing counts: 2^-inf = 0 everywhere
     float sums[V < 4 ? 4 : V], sum = 0.f;
 #pragma unroll
     for (int e = 0; e < (V < 4 ? 4 : V); ++e) sums[e] = 0.f;
 #pragma unroll
     for (int k = 0; k < NA; ++k) {
-      add_one(f[k], -mm);
+      fma_one(f[k], ex.s, ex.b);
 #pragma unroll
       for (int e = 0; e < V; ++e) f[k][e] = exp2_neg(f[k][e]);
       if constexpr (V == 8) {
@@ -383,7 +392,7 @@ relbias_fwd_kernel(const __grid_constant__ RbParams p) {
     float factor;
     if (WIDE) {
       const float2 all = rb_exchange(s_ex, turn, warps, p.cluster, rank, make_float2(m, sum), join_softmax);
-      factor = (m == -INFINITY ? 1.f : exp2_neg(m - all.x)) / all.y;
+      factor = (m == -INFINITY ? 1.f : exp2_neg((m - all.x) * kSteps)) / all.y;
       if (all.y == 0.f) factor = 0.f;
     } else {
       factor = sum == 0.f ? 0.f : __fdividef(1.f, sum);        // a row that nothing is visible to: zeros

@@ -426,3 +426,43 @@ def test_buckets_made_where_another_device_is_the_default():
     with torch.device("meta"):
         buckets = RelativeBuckets(32, 128, True)
     assert buckets.edges.device.type == "cpu" and torch.equal(buckets.edges, RelativeBuckets(32, 128, True).edges)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,cols", [(6, 200), (40, 1001), (6, 1500), (6, 20000)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_values_close_to_the_types_lowest(n, cols, dtype):
+    """Scores, table entries and masks at and near the ends of a type's range are numbers like others: a row of nothing but the lowest
+    value shares its 1, the largest of several far ones takes it all, and beside ordinary ones they are 0.  Where the exponents of a row are far
+    out, two of them are equal or so far apart that one exponential is 0: what is left are the sum's and the result's roundings."""
+    from hyc_lora_release_b200.operators import relative_bias_kernels as rb
+    t = DTYPES[dtype]
+    low = torch.finfo(t).min
+    buckets = rb.RelativeBuckets(32, 128, True)
+    scores, table, _, _ = _inputs(2, 3, n, cols, t, buckets, False, 0, n + cols)
+    scores[0, :, 0] = low                                # nothing else
+    scores[0, :, 1, ::2] = low                           # beside ordinary ones
+    scores[0, :, 2] = low / 2
+    scores[0, :, 2, 5] = low / 4                         # the largest of far ones
+    scores[1, :, 0] = -low / 2
+    scores[1, :, 0, 3] = -low * 0.75                     # far on the other side
+    mask = torch.zeros(2, 1, n, cols, dtype=t, device=DEV)
+    mask[1, :, 1] = low * 0.875
+    mask[1, :, 1, 7] = low * 0.6875                      # masks keep their order
+    mask[1, :, 2] = low
+    far = {(0, 0), (0, 2), (1, 0), (1, 1), (1, 2)}
+    one_value = table.clone()
+    one_value[:] = low                                   # .. and so does a table of them
+    for given_table, m, everywhere in ((table, mask, False), (table.float(), mask.float(), False), (one_value, None, True)):
+        s = torch.zeros_like(scores) if everywhere else scores
+        want, X = plain_forward(s, 1.0, given_table, buckets, m, False, 0)
+        got = rb.softmax_forward_relative_bias(s, 1.0, given_table, buckets, attention_mask=m)
+        for i in range(2):
+            for row in range(n):
+                x = torch.zeros_like(X[i, :, row]) if everywhere or (i, row) in far else X[i, :, row]
+                assert forward_close(got[i, :, row], want[i, :, row], x), (i, row)
+        assert bool((got.double().sum(-1) - 1).abs().max() < 0.02)
+    # -infinity is still nothing
+    scores[0, :, 0] = -math.inf
+    got = rb.softmax_forward_relative_bias(scores, 1.0, table, buckets)
+    assert bool((got[0, :, 0] == 0).all())
