@@ -47,7 +47,11 @@ inline int resident_blocks(K kern, int threads, size_t smem, int otherwise) {
   Entry& e = table[((reinterpret_cast<uintptr_t>(f) >> 4) ^ (uintptr_t)(threads >> 5) * 37u ^ (uintptr_t)(smem >> 10)) & 127];
   if (dev >= 0 && e.kern == f && e.threads == threads && e.smem == smem && e.device == dev) return e.blocks;
   int n = 0;
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, smem) != cudaSuccess || n < 1) return otherwise;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, smem) != cudaSuccess) {
+    (void)cudaGetLastError();      // (no error of the launch that follows)
+    return otherwise;
+  }
+  if (n < 1) return otherwise;
   e = {f, smem, threads, dev, n};
   return n;
 }

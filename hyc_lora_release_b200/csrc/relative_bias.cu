@@ -776,10 +776,8 @@ static void rb_fill(RbParams& p, const hyc_relative_bias* a, const RbPlan& r) {
 // the most dynamic shared memory of any plan: forward a mask and the bias of 16384 columns, backward the diagonals of 16 warps
 constexpr int kRbSmemFwd = (16384 + (16384 + 32 * kRbNarrowWarps) * 9 / 8 + 2) * 4, kRbSmemBwd = kRbMaxWarps * (1024 + 32) * 4;
 template <auto KERN>
-static int rb_launch(int most, const RbPlan& r, int64_t blocks, size_t smem, const RbParams& p, cudaStream_t st) {
+static int rb_launch(const RbPlan& r, int64_t blocks, size_t smem, const RbParams& p, cudaStream_t st) {
   if (blocks > 0x7fffffffll) return HYC_ERR_SHAPE;
-  const int rc = more_shared_memory<KERN>(most);
-  if (rc != HYC_OK) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)blocks);
   cfg.blockDim = dim3((unsigned)(32 * r.warps));
@@ -856,6 +854,8 @@ extern "C" HYC_API int hyc_softmax_relative_bias_fwd(const hyc_relative_bias* a,
     auto bytes = [&](int mask, int values) { return (size_t)(mask + values * 9 / 8 + 2) * sizeof(float); };
     const int block_warps = r.wide ? 1 : kRbNarrowWarps;      // warps with rows of their own
     const size_t most = bytes(one_mask ? width : 0, width + 32 * block_warps);
+    const int rs = more_shared_memory<kern>(kRbSmemFwd);      // (before the question: the answer counts on it)
+    if (rs != HYC_OK) return rs;
     const int64_t slots = (int64_t)num_sms() * resident_blocks(kern, 32 * r.warps, most, 1) / r.cluster;
     p.rows_per = rb_rows_per(a->batch * a->heads, (int)a->n, block_warps, slots < 1 ? 1 : slots, 3.f, a->causal != 0);
     const int rows = p.rows_per * block_warps;      // of a block
@@ -865,7 +865,7 @@ extern "C" HYC_API int hyc_softmax_relative_bias_fwd(const hyc_relative_bias* a,
     p.compact = few && distances < width;
     p.mask_staged = one_mask && !few ? width : 0;
     const size_t smem = bytes(p.mask_staged, p.compact ? distances : width + rows);
-    return rb_launch<kern>(kRbSmemFwd, r, a->batch * a->heads * p.chunks * r.cluster, smem, p, (cudaStream_t)stream);
+    return rb_launch<kern>(r, a->batch * a->heads * p.chunks * r.cluster, smem, p, (cudaStream_t)stream);
   });
 }
 
@@ -895,7 +895,8 @@ extern "C" HYC_API int hyc_softmax_relative_bias_bwd(const hyc_relative_bias* a,
       constexpr auto kern = relbias_bwd_kernel<decltype(elem), decltype(v)::value, decltype(nv)::value, decltype(wide)::value>;
       constexpr int V = decltype(v)::value, NV = decltype(nv)::value;
       const size_t smem = (size_t)r.warps * (size_t)rb_warp_floats(32 * V * NV, u.rows_per, RbRow<decltype(elem), V, NV, decltype(wide)::value>::BYTES) * sizeof(float);
-      return rb_launch<kern>(kRbSmemBwd, r, blocks, smem, p, (cudaStream_t)stream);
+      const int rs = more_shared_memory<kern>(kRbSmemBwd);
+      return rs != HYC_OK ? rs : rb_launch<kern>(r, blocks, smem, p, (cudaStream_t)stream);
     });
     if (rl != HYC_OK) return rl;
   }

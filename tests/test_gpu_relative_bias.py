@@ -466,3 +466,44 @@ def test_values_close_to_the_types_lowest(n, cols, dtype):
     scores[0, :, 0] = -math.inf
     got = rb.softmax_forward_relative_bias(scores, 1.0, table, buckets)
     assert bool((got[0, :, 0] == 0).all())
+
+
+FIRST_CALL = """
+import ctypes, torch
+from hyc_lora_release_b200.operators import relative_bias_kernels as rb
+driver = ctypes.CDLL("libcuda.so.1")
+
+class Params(ctypes.Structure):      # CUDA_KERNEL_NODE_PARAMS_v2
+    _fields_ = [("func", ctypes.c_void_p), ("grid", ctypes.c_uint * 3), ("block", ctypes.c_uint * 3), ("smem", ctypes.c_uint),
+                ("params", ctypes.c_void_p), ("extra", ctypes.c_void_p), ("kernel", ctypes.c_void_p), ("context", ctypes.c_void_p)]
+
+scores = torch.zeros(2, 32, 40, 8192, dtype=torch.bfloat16, device="cuda")
+mask, table, buckets = torch.zeros(1, 1, 1, 8192, device="cuda"), torch.zeros(32, 32, device="cuda"), rb.RelativeBuckets(32, 128, True)
+torch.cuda.synchronize()
+
+def launch():
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        rb.softmax_forward_relative_bias(scores, 1.0, table, buckets, attention_mask=mask)
+    raw, count = ctypes.c_void_p(graph.raw_cuda_graph()), ctypes.c_size_t()
+    assert driver.cuGraphGetNodes(raw, None, ctypes.byref(count)) == 0 and count.value == 1
+    node, p = (ctypes.c_void_p * 1)(), Params()
+    assert driver.cuGraphGetNodes(raw, node, ctypes.byref(count)) == 0
+    assert driver.cuGraphKernelNodeGetParams_v2(ctypes.c_void_p(node[0]), ctypes.byref(p)) == 0
+    return list(p.grid) + list(p.block) + [p.smem]
+
+first, second = launch(), launch()
+assert first == second, (first, second)
+print("same", first)
+"""
+
+
+@pytest.mark.gpu
+def test_the_first_call_is_cut_as_later_ones_are():
+    """In a process of its own: what one launch of long rows is, recorded on the first call and on the second."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "same" in r.stdout, r.stdout + r.stderr
