@@ -844,7 +844,8 @@ extern "C" HYC_API int hyc_linear_act_dpre(const void* dy, int64_t ld_dy, const 
 
 extern "C" HYC_API int hyc_linear_status(int* host_status) {
   if (host_status == nullptr) return HYC_ERR_NULL;
-  const cudaError_t e = cudaMemcpyFromSymbol(host_status, g_status, sizeof(int));
+  cudaError_t e = cudaDeviceSynchronize();      // (a copy alone would not wait for streams that do not wait for the default one)
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(host_status, g_status, sizeof(int));
   if (e != cudaSuccess) { hyc_set_last_cuda_error((int)e); cudaGetLastError(); return HYC_ERR_LAUNCH; }
   return HYC_OK;
 }

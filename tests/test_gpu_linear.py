@@ -306,3 +306,24 @@ def test_the_library_refuses_before_it_launches():
     need = lib.hyc_linear_act_dpre_workspace_bytes(64)
     assert need > 0 and dpre(p, 64, p, p, p, 8, 64, 0, 0, p, need - 1, None) == dpre(p, 64, p, p, p, 8, 64, 0, 0, None, need, None) == -5
     assert lib.hyc_linear_status(None) == -1
+
+
+@pytest.mark.gpu
+def test_the_status_waits_for_every_stream():
+    """Work on a stream that the default one does not wait for has ended when the status has been read."""
+    from hyc_lora_release_b200.operators import linear_kernels as lk
+    x, w, b, _, _, _ = inputs(64, 64, 64, torch.bfloat16, 1)
+    big = torch.randn(8192, 8192, device=DEV).to(torch.bfloat16)
+    stream, done = torch.cuda.Stream(), torch.cuda.Event()
+
+    def work(times):
+        with torch.cuda.stream(stream):
+            for _ in range(times):
+                big @ big
+            lk.linear_act_forward(x, w, b)
+            done.record()
+    work(1)                      # (memory and code are there: nothing else waits for the device)
+    torch.cuda.synchronize()
+    work(60)                     # tens of milliseconds
+    lk.raise_on_device_errors()
+    assert done.query()
