@@ -32,8 +32,14 @@ def linear_act_backward(dy, x, weight, activation="none", pre=None, needs_grad=(
 
 
 def raise_on_device_errors(device=None):
-    """Waits for the device and raises if a bounded wait inside these kernels gave up on it since the library was loaded."""
-    status = host.linear_status(torch.cuda.current_device() if device is None else torch.device(device).index or 0)
+    """Waits for the device (default: the current one) and raises if a bounded wait inside these kernels gave up on it since the library
+    was loaded."""
+    if isinstance(device, (str, torch.device)):
+        device = torch.device(device)
+        if device.type != "cuda":
+            raise ValueError("expected a CUDA device, got %s" % device)
+        device = device.index
+    status = host.linear_status(torch.cuda.current_device() if device is None else int(device))
     if status != 0:
         raise HycError("linear kernels: %s" % {1: "TMA producer wait timed out", 2: "MMA issuer wait timed out", 3: "epilogue wait timed out"}
                        .get(status, "status %d" % status))

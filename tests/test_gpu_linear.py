@@ -327,3 +327,21 @@ def test_the_status_waits_for_every_stream():
     work(60)                     # tens of milliseconds
     lk.raise_on_device_errors()
     assert done.query()
+
+
+def test_the_status_is_of_the_device_that_is_meant(monkeypatch):
+    from hyc_lora_release_b200.operators import linear_kernels as lk
+    asked = []
+
+    class Host:
+        @staticmethod
+        def linear_status(device):
+            asked.append(device)
+            return 0
+    monkeypatch.setattr(lk, "host", Host)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 3)
+    for device in (None, "cuda", torch.device("cuda"), "cuda:0", torch.device("cuda", 2), 1):
+        lk.raise_on_device_errors(device)
+    assert asked == [3, 3, 3, 0, 2, 1]
+    with pytest.raises(ValueError):
+        lk.raise_on_device_errors("cpu")
