@@ -44,12 +44,18 @@ struct Shape { int R, C, K; };
 
 // ---- activations, fp32
 __device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
-// erfc(|x| / sqrt 2) / 2 = q(t) e^(-x^2 / 2), t = 1 / (1 + p |x| / sqrt 2): the rational approximation 7.1.26 of Abramowitz and Stegun's
-// Handbook, off by 7.5e-8 at most (half of erf's 1.5e-7).  x Phi(x) = max(x, 0) - |x| erfc(..) / 2, with no cancellation on either side.
+// erfc(|x| / sqrt 2) / 2 = q(t) e^(-x^2 / 2), t = 1 / (1 + 0.36 |x| / sqrt 2).  q / t is a polynomial of degree 6, fitted for the least maximum of the
+// relative error over |x| < 14, weighted towards 0 (a linear program over its Chebyshev coefficients): with fp32's roundings q is off by 4.9e-6 of
+// itself, the tail by 2.1e-7.  x Phi(x) = max(x, 0) - |x| erfc(..) / 2, with no cancellation on either side.
 __device__ __forceinline__ float normal_tail(float x, float& density) {      // density: e^(-x^2 / 2)
   const float ax = fabsf(x);
-  const float t = __fdividef(1.f, fmaf(0.3275911f * 0.70710678118654752f, ax, 1.f));
-  const float q = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f), 0.5f * 1.421413741f), 0.5f * -0.284496736f), 0.5f * 0.254829592f);
+  const float t = __fdividef(1.f, fmaf(0.36f * 0.70710678118654752f, ax, 1.f));
+  float q = fmaf(t, -0.08069140564f, 0.277714377f);
+  q = fmaf(t, q, -0.1709972366f);
+  q = fmaf(t, q, 0.2089158673f);
+  q = fmaf(t, q, 0.05609946922f);
+  q = fmaf(t, q, 0.1078153617f);
+  q = t * fmaf(t, q, 0.1011436123f);
   density = __expf(-0.5f * x * x);
   return q * density;
 }

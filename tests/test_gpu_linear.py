@@ -345,3 +345,19 @@ def test_the_status_is_of_the_device_that_is_meant(monkeypatch):
     assert asked == [3, 3, 3, 0, 2, 1]
     with pytest.raises(ValueError):
         lk.raise_on_device_errors("cpu")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("t", [4, 600])
+def test_gelu_far_out_on_the_left(t, dtype):
+    """x Phi(x) for x from -14 to -1, where it is small: relative to itself.  Before the one rounding: the tail's rational function 2^-17;
+    the exponential's argument, up to 90 and rounded three times, 3 * 90 * 2^-24 < 2^-15; its two units, the quotient's and the products' 2^-20."""
+    from hyc_lora_release_b200.operators import linear_kernels as lk
+    k = 512
+    x = torch.linspace(-14, -1, t * k).view(t, k).to(DTYPES[dtype]).to(DEV)
+    y, _ = lk.linear_act_forward(x, torch.eye(k, dtype=x.dtype, device=DEV), None, "gelu")
+    want = x.double() * torch.special.erfc(-x.double() / 2 ** 0.5) / 2
+    f = torch.finfo(x.dtype)
+    # (a result below fp32's smallest normal number may be 0)
+    assert bool(((y.double() - want).abs() <= want.abs() * (f.eps / 2 + 2.0 ** -14) + f.smallest_normal * f.eps + 2.0 ** -126).all())
