@@ -30,13 +30,13 @@ static Tensor head_view(const Tensor& t_in, int64_t (&stride)[3]) {
   }
   return t;
 }
-// a table of `rows` angles as [rows, >= half]
+// a table of `rows` angles as [rows, >= half], with a row stride that the library takes (expanded and overlapping rows are copied)
 static Tensor angle_table(const Tensor& t_in, int64_t half, const char* what) {
   TORCH_CHECK_VALUE(t_in.dim() >= 2 && t_in.numel() == t_in.size(-2) * t_in.size(-1) && t_in.size(-1) >= half, what,
                     " must be a [positions, >= rotary_dim / 2] table, got shape ", t_in.sizes());
   Tensor t = t_in.dim() == 2 ? t_in : t_in.reshape({t_in.size(-2), t_in.size(-1)});
   if (elem_type(t.scalar_type()) < 0) t = t.to(at::kFloat);
-  if (t.numel() > 0 && (t.stride(1) != 1 || !on16(t) || (t.size(0) > 1 && t.stride(0) % (16 / t.element_size()) != 0)))
+  if (t.numel() > 0 && (t.stride(1) != 1 || !on16(t) || (t.size(0) > 1 && (t.stride(0) < half || t.stride(0) % (16 / t.element_size()) != 0))))
     t = t.narrow(1, 0, half).clone(at::MemoryFormat::Contiguous);
   return t;
 }

@@ -302,3 +302,18 @@ def test_the_library_refuses_before_it_launches():
     for change in (dict(x=(0, p + 2)), dict(weight=(1, p + 8)), dict(out=(1, p + 4)), dict(x_stride=(2, 68)), dict(ld_sin=68, table_type=0), dict(sin_t=p + 4)):
         assert call(batch=1, **change) == -4, change
     assert call(backward=True) == -5                                       # no workspace
+
+
+@pytest.mark.gpu
+def test_tables_that_are_one_row_for_all_positions():
+    """Expanded tables (row stride 0) and tables whose rows overlap."""
+    from hyc_lora_release_b200.operators import qk_norm_kernels as qn
+    q, k, w, dy = _inputs(2, 6, 3, 2, 64, torch.bfloat16, packed=False, seed=9)
+    for t in DTYPES.values():
+        cos, sin = _tables(6, 64, t)
+        for c, s in ((cos[3:4].expand(6, 64), sin[3:4].expand(6, 64)), (cos[3:4].expand(6, 64), sin),
+                     (cos.reshape(-1).as_strided((6, 32), (16, 1)), sin.reshape(-1).as_strided((6, 32), (16, 1)))):
+            _check(q, k, w, dy, c, s, None, 64)
+            got = qn.qk_norm_rope_forward(q, k, *w, c, s, EPS)
+            want = qn.qk_norm_rope_forward(q, k, *w, c.contiguous(), s.contiguous(), EPS)
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
