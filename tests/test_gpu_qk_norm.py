@@ -317,3 +317,43 @@ def test_tables_that_are_one_row_for_all_positions():
             got = qn.qk_norm_rope_forward(q, k, *w, c, s, EPS)
             want = qn.qk_norm_rope_forward(q, k, *w, c.contiguous(), s.contiguous(), EPS)
             assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def _weight_gradients_close(got, want, mag, chain):
+    """-> whether they are within the bound, the bound"""
+    f = torch.finfo(got.dtype)
+    bound = f.eps / 2 * (want.abs() + chain * mag) + chain * mag + f.smallest_normal * f.eps
+    return bool(((got.double() - want).abs() <= bound).all()), bound
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,b,m,hq,hk,d,rot", [("bf16", 2, 1500, 32, 32, 128, 128), ("bf16", 4, 2048, 32, 8, 128, 128), ("fp16", 3, 1333, 12, 12, 64, 32),
+                                                   ("fp32", 2, 1500, 24, 8, 96, 96), ("fp32", 1, 2000, 8, 2, 512, 512), ("bf16", 2, 3000, 7, 1, 80, 80)])
+def test_weight_gradients_of_many_tokens(dtype, b, m, hq, hk, d, rot):
+    """Sums over all tokens and heads, as the kernel takes them: the grid has at least two blocks per 32 SMs and tensor, of eight warps that
+    share a tensor's heads evenly but for one token's each, and a lane adds up the heads of its place in the warp; then the warp's
+    heads (32 at most), eight warps, and the blocks, every 32nd by a thread (10 at most) and five steps of a tree.  In roundings of 2^-24 relative to the
+    magnitudes, on top of a head's own chain.  The gradients are far above that: half of one, or one without an eightieth of the tokens, would not pass."""
+    from hyc_lora_release_b200.operators import qk_norm_kernels as qn
+    t = DTYPES[dtype]
+    q, k, w, dy = _inputs(b, m, hq, hk, d, t, packed=True, seed=m)
+    for x, g in ((q, dy[0]), (k, dy[1])):      # gradients that follow the heads: the sums grow with the number of tokens
+        g.copy_(g.float() + x.float())
+    cos, sin = _tables(m, rot, torch.float32)
+    one, zero = torch.ones_like(cos), torch.zeros_like(sin)
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    for c_table, s_table in ((cos, sin), (one, zero)):
+        c, s = _angles(c_table, s_table, None, b, m, rot)
+        grads = qn.qk_norm_rope_backward(*dy, q, k, *w, c_table, s_table, EPS, rotary_dim=rot)
+        for i, x in enumerate((q, k)):
+            _, want, _, mag = plain_backward(dy[i], x, w[i], c, s, rot)
+            heads = x.shape[0] * x.shape[1] * x.shape[2]
+            lane = heads / (sms // 32 * 2 * 8) + x.shape[2]      # (a warp's heads, all in one place: more than a lane has)
+            chain = FP32_CHAIN + (lane + 32 + 8 + 10 + 5) * 2.0 ** -24
+            fits, bound = _weight_gradients_close(grads[2 + i], want, mag, chain)
+            assert fits
+            if s_table is zero:
+                assert bool((bound < want.abs() / 80).all())
+                assert not _weight_gradients_close(grads[2 + i] / 2, want, mag, chain)[0]
+                share = plain_backward(dy[i][:, :m // 80 + 1], x[:, :m // 80 + 1], w[i], c[:, :m // 80 + 1], s[:, :m // 80 + 1], rot)[1]
+                assert not _weight_gradients_close(grads[2 + i], want + share, mag, chain)[0]
