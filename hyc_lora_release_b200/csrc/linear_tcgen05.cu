@@ -10,7 +10,7 @@
 // (up to 1.5 with one to four tokens); a second product with what the rounding took would double the work.
 //
 // Two kernels, both fed by TMA (128-byte swizzle, 64-wide k-blocks; what lies outside of an operand arrives as zero, so that any number of
-// rows and any multiple of 8 columns is right), every wait bounded (hyc_linear_status):
+// rows and any multiple of 8 columns is right), every wait bounded (hyc_linear_status; tc_settle before a CTA leaves):
 //   tiles    persistent CTA pairs, 256 x 256 or 256 x 128 results per pair by tcgen05.mma.cta_group::2, two accumulators, so that the
 //            epilogue of one tile overlaps the main loop of the next
 //   slices   few rows or few tiles: one tile of 128 result COLUMNS x up to 256 rows per CTA (256 per CTA pair), the columns on the lanes of
@@ -349,6 +349,7 @@ linear_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
   // both CTAs are done with each other's barriers and tensor memory before either leaves
   tc_fence_before();
   __syncthreads();
+  tc_settle(abort_flag);
   cluster_sync_all();
   if (warp == 1) {
     tc_fence_after();
@@ -564,6 +565,7 @@ linear_slices_kernel(const __grid_constant__ CUtensorMap map_c, const __grid_con
   }
   tc_fence_before();
   __syncthreads();
+  tc_settle(flag);
   if (clustered) cluster_sync_all();      // nobody leaves while a peer may still read its partial sums or use its barriers
   if (warp == 1) {
     tc_fence_after();

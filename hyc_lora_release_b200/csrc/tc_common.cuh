@@ -159,6 +159,19 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, v
   }
   return false;
 }
+// By all threads of a CTA after its last __syncthreads(), before it leaves or gives tensor memory back.  Where a wait gave up, copies into its
+// shared memory and MMAs may still be under way, some of them counted on a barrier of the peer: a millisecond is hundreds of times what
+// they take.  (Bounded by its iterations, too.)
+__device__ __forceinline__ void tc_settle(const volatile int* abort_flag) {
+  if (*abort_flag == 0) return;
+  uint64_t begun, now;
+  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(begun));
+  for (int i = 0; i < 100000; ++i) {
+    __nanosleep(200);
+    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
+    if (now - begun > 1000000u) break;
+  }
+}
 // a tile into this CTA's shared memory; the bytes are counted on the barrier at shared::cluster address `bar`,
 // which in the pair form may belong to the other CTA of the pair (that is what .cta_group::2 permits)
 template <bool PAIR>
