@@ -261,9 +261,10 @@ __device__ __forceinline__ uint32_t at_setup(const AttnParams& p, const Bars& ba
   if (warp == 2 && lane < p.tiles) bar.cls[lane] = (uint8_t)class_of(p, b, h, qt, lane);
   return at_ready(bar);
 }
-__device__ __forceinline__ void at_teardown(int warp, uint32_t tmem_base) {
+__device__ __forceinline__ void at_teardown(const Bars& bar, int warp, uint32_t tmem_base) {
   tc_fence_before();
   __syncthreads();
+  tc_settle(bar.abort_flag);
   if (warp == 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512) : "memory");
@@ -535,7 +536,7 @@ attn_fwd_kernel(const __grid_constant__ FwdMaps maps, const AttnParams p) {
       }
     }
   }
-  at_teardown(warp, tmem);
+  at_teardown(bar, warp, tmem);
 }
 
 // ------------------------------------------------------------------ backward, q side
@@ -739,7 +740,7 @@ attn_bwd_q_kernel(const __grid_constant__ BwdQMaps maps, const AttnParams p) {
       flush_clipped(R, p.out0 + (int64_t)b * p.M * ld, qt * TILE + quad * 32, p.M, ld, h * TILE + 32 * part, (int)ld, lane);
     }
   }
-  at_teardown(warp, tmem);
+  at_teardown(bar, warp, tmem);
 }
 
 // ------------------------------------------------------------------ backward, kv side
@@ -888,7 +889,7 @@ attn_bwd_kv_kernel(const __grid_constant__ BwdKvMaps maps, const AttnParams p) {
       if (any) ++used;
     }
   }
-  at_teardown(warp, tmem);
+  at_teardown(bar, warp, tmem);
 }
 
 // ------------------------------------------------------------------ host side

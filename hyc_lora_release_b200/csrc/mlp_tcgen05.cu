@@ -593,6 +593,7 @@ mlp_gemm_kernel(const __grid_constant__ Maps maps, const Params p) {
   // both CTAs are done with each other's barriers and tensor memory before either leaves
   tc_fence_before();
   __syncthreads();
+  tc_settle(abort_flag);
   if (PAIR) cluster_sync_all();
   if (warp == 1) {
     tc_fence_after();

@@ -186,6 +186,7 @@ skinny_kernel(const __grid_constant__ Args a) {
   }
   tc_fence_before();
   __syncthreads();
+  tc_settle(abort_flag);
   if (warp == 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");

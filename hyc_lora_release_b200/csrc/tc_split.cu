@@ -381,6 +381,7 @@ split_gemm_kernel(const __grid_constant__ Maps maps, const Params p, int split, 
 
   tc_fence_before();
   __syncthreads();
+  tc_settle(abort_flag);
   if (PAIR || split > 1) cluster_sync_all();      // nobody leaves while a peer may still read its partial sums
   if (warp == 1) {
     tc_fence_after();
