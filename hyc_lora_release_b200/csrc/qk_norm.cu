@@ -97,7 +97,7 @@ __device__ __forceinline__ void qk_angles(const QkParams& p, int b, int m, const
   } else {
     const float nan = __int_as_float(0x7fc00000);
 #pragma unroll
-    for (int e = 0; e < N; ++e) { a.c[e] = both(l.turned() ? nan : 1.f); a.s[e] = both(l.turned() ? nan : 0.f); }
+    for (int e = 0; e < N; ++e) a.c[e] = a.s[e] = both(nan);      // (channels that are not turned do not look)
   }
 #pragma unroll
   for (int e = 0; e < N; ++e) a.ns[e] = a.s[e] ^ 0x8000000080000000ull;
@@ -247,8 +247,8 @@ qk_norm_fwd_kernel(const __grid_constant__ QkParams p) {
 #pragma unroll
       for (int e = 0; e < N; ++e) {
         const f32x2 n1 = mul2f(mul2f(f1[e], rr), w1[e]), n2 = mul2f(mul2f(f2[e], rr), w2[e]);
-        f1[e] = fma2f(n2, a.ns[e], mul2f(n1, a.c[e]));
-        f2[e] = fma2f(n1, a.s[e], mul2f(n2, a.c[e]));
+        f1[e] = l.turned() ? fma2f(n2, a.ns[e], mul2f(n1, a.c[e])) : n1;      // (not by way of n2 * 0: it may be infinite)
+        f2[e] = l.turned() ? fma2f(n1, a.s[e], mul2f(n2, a.c[e])) : n2;
       }
       if (l.live() && left > 0) {
         st_pairs(dst, f1);
@@ -300,7 +300,8 @@ qk_norm_bwd_kernel(const __grid_constant__ QkParams p) {
       feed.send();
 #pragma unroll
       for (int e = 0; e < N; ++e) {
-        const f32x2 u = fma2f(g2[e], a.s[e], mul2f(g1[e], a.c[e])), v = fma2f(g1[e], a.ns[e], mul2f(g2[e], a.c[e]));
+        const f32x2 u = l.turned() ? fma2f(g2[e], a.s[e], mul2f(g1[e], a.c[e])) : g1[e];
+        const f32x2 v = l.turned() ? fma2f(g1[e], a.ns[e], mul2f(g2[e], a.c[e])) : g2[e];
         ss = fma2f(f1[e], f1[e], fma2f(f2[e], f2[e], ss));
         sg = fma2f(mul2f(u, f1[e]), w1[e], fma2f(mul2f(v, f2[e]), w2[e], sg));
         g1[e] = u; g2[e] = v;

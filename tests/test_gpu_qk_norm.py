@@ -357,3 +357,24 @@ def test_weight_gradients_of_many_tokens(dtype, b, m, hq, hk, d, rot):
                 assert not _weight_gradients_close(grads[2 + i] / 2, want, mag, chain)[0]
                 share = plain_backward(dy[i][:, :m // 80 + 1], x[:, :m // 80 + 1], w[i], c[:, :m // 80 + 1], s[:, :m // 80 + 1], rot)[1]
                 assert not _weight_gradients_close(grads[2 + i], want + share, mag, chain)[0]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("d,rot", [(64, 32), (80, 32), (96, 48), (128, 64), (320, 160)])
+def test_infinities_in_channels_that_are_not_turned(dtype, d, rot):
+    """Behind rotary_dim every channel is on its own: an infinity there is in no other channel's result, nor in another's weight gradient."""
+    from hyc_lora_release_b200.operators import qk_norm_kernels as qn
+    t = DTYPES[dtype]
+    cos, sin = _tables(7, rot, torch.float32)
+    for at in range(rot, d):
+        q, k, w, dy = _inputs(1, 7, 3, 2, d, t, packed=False, seed=d)
+        q[0, 2, 1, at] = float("inf")
+        dy[1][0, 3, 0, at] = float("inf")
+        out = qn.qk_norm_rope_forward(q, k, *w, cos, sin, EPS, rotary_dim=rot)[0][0, 2, 1]
+        want = torch.zeros(d, device=DEV)
+        want[at] = float("nan")                          # (a root of infinity: everything else is 0)
+        assert torch.equal(out.isnan(), want.isnan()) and bool((out[~want.isnan()] == 0).all())
+        dw = qn.qk_norm_rope_backward(*dy, q, k, *w, cos, sin, EPS, rotary_dim=rot)[3]
+        others = torch.arange(d, device=DEV) != at
+        assert bool(dw[others].isfinite().all()) and not bool(dw[at].isfinite())
