@@ -17,10 +17,12 @@
 //            tensor memory and the rows in its columns (a product of one row costs N = 16, not 128), K shared by the CTAs or pairs of a
 //            cluster, whose partial sums meet in distributed shared memory in a fixed order
 //
-// B200, bf16, us of one launch alone (share of the measured burst rate or copy peak): tiles 2048 x 4096 -> 11008 with gelu and pre 112-127 on different boxes
-// (0.99-0.88), its dx 111-127, dW 104-119, 8192 x 4096 -> 14336 573-609, with gelu and pre 604-640; the tensor pipe is busy 92 % of the cycles.  Slices: 1 x 4096
-// -> 11008 20 (0.68 of the copy peak), 1 x 4096 -> 4096 13, 128 x 4096 -> 4096 17-18, 333 x 11008 -> 4096 32: bound by the weight's bytes and
-// the start and end of a launch (about 6 us), from 200 rows on by operands from L2.  dpre of 2048 x 11008 with silu 25 (0.83).
+// B200, bf16, us of one launch alone, on different boxes (share of the measured burst rate or copy peak): tiles 2048 x 4096 -> 11008 with gelu and pre 112-127
+// (0.99-0.88), its dx 111-128, dW 104-120, 8192 x 4096 -> 14336 573-609, with gelu and pre 604-640; the tensor pipe is busy 92 % of the cycles.  In a row of
+// passes, under the power cap: 154, 125, 125, 719 and 744-768.  Slices, in a row of passes: 1 x 4096 -> 11008 19 (0.74 of the copy peak), 1 x 4096
+// -> 4096 10, 128 x 4096 -> 4096 16, 333 x 11008 -> 4096 38 (alone 22, 13, 17, 31-35): bound by the weight's bytes and the start and end of a launch
+// (about 6 us), from 200 rows on by operands from L2.  dpre of 2048 x 11008 with silu 25 alone (0.83).  Backward of 1 to 128 tokens, 4096 -> 11008: dx 20-24
+// (0.67-0.58), dW 38-39 (0.36): its 90 MB of results leave through the epilogue, eight warps per SM that take 32 x 32 of them at a time.
 #include "tc_common.cuh"
 #include "elem.cuh"
 #include <type_traits>

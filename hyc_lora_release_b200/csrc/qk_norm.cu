@@ -15,9 +15,10 @@
 // warps to hide the memory: 4 x 2048 tokens of 32 + 8 heads 36 against 33 us, backward 60 against 51).  Backward's gradients of the weights: per
 // lane over all its heads, then per block in a fixed order, then one small launch over the blocks: the same bits on every run.
 //
-// B200, bf16, heads of 128, q and k of 32 + 8 heads: 4 x 2048 tokens forward 26 us (6.4 TB/s, 0.98 of the copy peak), backward 42 us (6.0 TB/s); 2048
-// tokens of 32 + 32 heads 14 us and 20 + 5 us.  fp32 heads of 96 18 and 26 us for 4096 tokens of 24 + 8 (0.86, 0.88).  4 x
-// 2048 tokens of 32 + 8 heads of 80, six of them per warp: 25 and 42 us (0.64, 0.57; four per warp, on lanes by powers of two: 31 and 43).
+// B200, us in a row of passes, share of the copy peak, forward / backward with the weights' gradients (5 of them the second launch): bf16, heads of 128,
+// 4 x 2048 tokens of 32 + 8 heads 30 (0.84) / 47 (0.82), 2048 tokens of 32 + 32 heads 15 (0.70) / 22 (0.69); alone they take 26 to 32 and 20 to 21 + 5 on
+// different boxes.  fp32 heads of 96, 4096 tokens of 24 + 8: 21 (0.74) / 31 (0.75).  4 x 2048 tokens of 32 + 8 heads of 80, six of them per
+// warp: 24 (0.66) / 42 (0.57); four per warp, on lanes by powers of two: 31 and 43.
 #include "elem.cuh"
 #include <type_traits>
 

@@ -19,14 +19,17 @@
 // running sum of each diagonal moves one column to the right: within a lane's V columns that is an operand of the addition, between
 // lanes one shuffle per V elements, and what leaves the warp's last column is put aside in shared memory.  After the last row the
 // sums of SPAN + R - 1 diagonals are there, and each bucket's are added up: no atomics, the same bits on every run.  A small
-// second launch adds the warps' sums per head, in 64 bits.  Buckets hold long ranges whose sums nearly cancel: where warps share a row (few
-// rows, nothing averages out) the row's product sum and the buckets' are in 64 bits too (in 32 the table's gradient of single tokens was
-// up to 15 times as far off as the formula's in 32 bits with sums in 64; everywhere it would cost 2 to 7 %, and there rows average it out).
+// second launch adds the warps' sums per head, in 64 bits.  Buckets hold long ranges whose sums nearly cancel: where warps share a row (WIDE: rows
+// beyond a warp's span, and rows of more than 512 columns of which there are fewer than eight per SM) the row's product sum and the
+// buckets' are in 64 bits too (in 32 the table's gradient of single tokens over 1277 columns and more was up to 15 times as far off as the formula's
+// in 32 bits with sums in 64; everywhere it would cost 2 to 7 %).  Of many rows the sums average out; rows of up to 512 columns keep 32
+// bits even if there is one of them: over 25 inputs each of 37 to 512 columns the gradient is 0.6 to 1.4 times as far off as that formula's (median).
 //
-// B200, us, share of the copy peak, forward / backward (without the second launch, 5 us): bf16 [4,32,512,512] 29 (padding, 0.70) / 42 (0.73);
-// [1,32,2048,2048] 90 (0.91) / 139 (0.89), causal 79 (0.78) / 106 (0.77); [2,32,696,696] causal 35 (0.41) / 32 (0.59); fp32 [4,16,1000,1000] 87 (0.90) /
-// 117 (1.0); fp16 [2,32,1002,1002] 54 (0.73) / 69 (0.85), [2,32,1001,1001] causal 64 (0.46) / 82 (0.48): single elements per access cost instructions.
-// Forward is bound by instruction issue (15 per element, exponentials a third of their unit), backward by the latency of its rows.
+// B200, us in a row of passes, share of the copy peak, forward / backward (with the second launch, 5 us): bf16 [4,32,512,512] 27 (padding, 0.77) / 47
+// (0.66); [1,32,2048,2048] 103 (0.80) / 146 (0.84), causal 85 (0.72) / 112 (0.73); [2,32,696,696] causal 32 (0.45) / 37 (0.51); fp32 [4,16,1000,1000] 90
+// (0.87) / 126 (0.93); fp16 [2,32,1002,1002] 50 (0.78) / 73 (0.80), [2,32,1001,1001] causal 62 (0.48) / 87 (0.45): single elements per access cost
+// instructions.  Forward is bound by instruction issue (15 per element, exponentials a third of their unit), backward by the latency of its rows.
+// (Figures of single choices, at the places, are launches alone.)
 #include "elem.cuh"
 #include <type_traits>
 

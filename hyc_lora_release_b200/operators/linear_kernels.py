@@ -26,7 +26,8 @@ def linear_act_forward(x, weight, bias=None, activation="none", residual=None, s
 def linear_act_backward(dy, x, weight, activation="none", pre=None, needs_grad=(True, True, True)):
     """-> (grad_x, grad_weight, grad_bias), None where ``needs_grad`` does not ask for one (frozen weights: ``(True, False, False)``).
     ``pre`` as forward saved it (not needed without an activation); the residual's gradient is ``dy`` itself.  ``dy * act'(pre)`` is
-    rounded to the operands' type before its two products, its column sums, the bias gradient, are not."""
+    rounded to the operands' type before its two products, so that grad_x and grad_weight carry about 1.4 times the error of their own
+    rounding (up to 1.5 with one to four tokens); its column sums, the bias gradient, are taken of the unrounded values."""
     need_x, need_w, need_b = needs_grad
     return host.linear_act_backward(dy, x, weight, _act(activation), pre, bool(need_x), bool(need_w), bool(need_b))
 

@@ -46,7 +46,8 @@ def softmax_forward_relative_bias(scores, scale, table, buckets, attention_mask=
     [b or 1, h or 1, n or 1, S] each of one of these types; buckets: a ``RelativeBuckets``.  q_offset: position of the first row among
     the columns (S - n for queries at the end of a cache; a single token is n = 1).  causal: row i sees columns up to i + q_offset;
     what lies behind is not read and is 0 in the result.  A row that sees nothing (no column, or -infinity everywhere) is 0; where the
-    mask is the type's lowest value instead, it shares its 1 among the columns, as the sum says.  fp32 inside, rounded once.
+    mask is the type's lowest value instead, it shares its 1 among the columns, as the sum says: values up to the ends of a type's range are
+    numbers like others, in scores, table and mask.  fp32 inside, rounded once.
     ``inplace`` overwrites ``scores`` (which must then be contiguous) and returns them."""
     return host.softmax_relative_bias_forward(scores, float(scale), table, buckets.edges, buckets.bidirectional, attention_mask, bool(causal),
                                               int(q_offset), bool(inplace))
@@ -55,5 +56,5 @@ def softmax_forward_relative_bias(scores, scale, table, buckets, attention_mask=
 def softmax_backward_relative_bias(a, grad_a, scale, buckets, causal=False, q_offset=0):
     """-> (grad_scores, grad_table) for the probabilities ``a`` and their gradient: ``ds = a * (grad_a - rowsum(a * grad_a))``,
     grad_scores = ds * scale in the type of ``a``, grad_table fp32 [num_buckets, h] = ds summed over batch, rows and the distances of a
-    bucket, in a fixed order.  ``scale``, ``buckets``, ``causal`` and ``q_offset`` as forward had them."""
+    bucket, in a fixed order, rows that lie behind the last column (causal, i + q_offset >= S) among them.  ``scale``, ``buckets``, ``causal`` and ``q_offset`` as forward had them."""
     return host.softmax_relative_bias_backward(a, grad_a, float(scale), buckets.edges, buckets.bidirectional, bool(causal), int(q_offset))
